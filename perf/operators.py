@@ -113,6 +113,10 @@ def prepare(case, seed):
         st["logprobs"], st["entropy"] = torch.empty(rows, **f32), torch.empty(rows, **f32)
         st["top_logprobs"] = torch.empty(rows, k, **f32)
         st["top_ids"] = torch.empty(rows, k, dtype=torch.int32, device="cuda")
+        if own:
+            from foundry_b200 import ops
+
+            st["ws"] = ops.LogprobWorkspace()
         return st
     n_q, n_kv, lens = case["n_q"], case["n_kv"], _lengths(case)
     if case["op"] == "prefill":
@@ -152,16 +156,15 @@ def prepare(case, seed):
     st["k_cache"], st["v_cache"] = normal(blocks, n_kv, PAGE, D), normal(blocks, n_kv, PAGE, D)
     st["q"] = normal(b, n_q, D, scale=1.5)
     st["out"] = torch.empty(b, n_q, D, dtype=torch.bfloat16, device="cuda")
-    if own:  # what a serving loop keeps between steps: the batch's plan and the workspace of its partial results
+    if own:  # what a serving loop keeps between steps: the batch's plan and a workspace
         from foundry_b200 import ops
 
+        partials = 0
         if case["op"] == "prefix":
             st["plan"] = ops.PrefixPlan([case["rows"]] * case["groups"], [case["prefix_pages"]] * case["groups"],
                                         n_q, n_kv, st["block_tables"].shape[1])
-            st["ws"] = ops.DecodeWorkspace(b, n_q, st["plan"].parts)
-        else:
-            splits, _ = ops.window_splits(b, n_kv, case["window"], case["sinks"], st["block_tables"].shape[1])
-            st["ws"] = ops.DecodeWorkspace(b, n_q, splits)
+            partials = st["plan"].partials
+        st["ws"] = ops.SpanWorkspace(partials)
     return st
 
 
@@ -254,9 +257,10 @@ def run(st):
         return ops.window_prefill_attention(st["q"], st["k"], st["v"], st["out"], st["cu_seqlens"], st["tile_seq"],
                                             st["tile_start"], st["n_q"], st["n_kv"], st["window"], st["sinks"])
     if not st["k"]:
-        ops.token_logprobs(st["logits"], st["ids"], st["logprobs"], st["entropy"])
+        ops.token_logprobs(st["logits"], st["ids"], st["logprobs"], st["entropy"], ws=st["ws"])
         return [st["logprobs"], st["entropy"]]
-    ops.token_logprobs(st["logits"], st["ids"], st["logprobs"], st["entropy"], st["top_logprobs"], st["top_ids"])
+    ops.token_logprobs(st["logits"], st["ids"], st["logprobs"], st["entropy"], st["top_logprobs"], st["top_ids"],
+                       ws=st["ws"])
     return [st["logprobs"], st["entropy"], st["top_logprobs"], st["top_ids"]]
 
 
