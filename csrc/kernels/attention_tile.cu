@@ -1,0 +1,530 @@
+// Attention of 128-query tiles against a list of 128-key tiles on the tcgen05
+// tensor cores (head_dim 128, bf16, GQA). Two kernels share the body:
+//
+//   fb_window_prefill_q{1,2}  packed prompts; key j is visible to the query at
+//                             position i iff j <= i and (j > i - window or
+//                             j < sinks); writes bf16 rows
+//   fb_prefix_attn_q{1,2}     a decode batch against pages that a group of its
+//                             sequences shares: the group's queries x G heads
+//                             of one KV head are the rows of the tile; writes
+//                             unnormalised fp32 partials and (max, sum) for
+//                             the join in attention_span.cu
+//
+// Per key tile and 128-row query tile:
+//   S = Q K^T          tcgen05.mma M=128 N=128 K=128, both from shared memory
+//   softmax            one thread per row: the row's 128 scores are read from
+//                      TMEM once into registers; running max m, sum l;
+//                      p = exp2(s - m) goes back to TMEM as bf16 over S
+//   O += P V           tcgen05.mma with P from TMEM (no shared-memory traffic
+//                      for it), V MN-major from the image that TMA wrote
+// A CTA holds QT query tiles: with QT = 2 they share every K/V tile and take
+// turns, the tensor cores working on one tile's products while the other's
+// 128 threads do its softmax; QT = 1 (half the shared memory and TMEM, two
+// CTAs per SM) is for work with no second tile. TMEM: QT x (128 columns S/P +
+// 128 columns O).
+//
+// The MMA thread issues P_t V_i and then Q_t K_{i+1}, which overwrites P_t's
+// columns: MMAs of one CTA execute in issue order. The commit behind Q_t K_{i+1}
+// therefore also covers P_t V_i, so a softmax thread that has seen S_{i+1} may
+// rescale O. A row's max moves only when a tile's max exceeds it by more than
+// 8 (log2 units; p stays below 256, exact in the fp32 sum), so O is rarely
+// rescaled.
+//
+// p is rounded to bf16 for the second product (relative 2^-9 per term, with
+// random signs), the sum l and both products accumulate in fp32.
+//
+// Roles: warps [0, 4 QT) softmax and epilogue, then one TMA warp, one MMA warp.
+// No TMA multicast; every wait bounded (fb_common.cuh).
+#include "attn_tile.cuh"
+
+FB_DEFINE_STATUS
+
+using namespace fbk;
+
+namespace {
+
+constexpr int D = 128;
+constexpr int PAGE = 64;
+constexpr int BQ = 128;              // query rows per tile
+constexpr int BK = 128;              // keys per tile
+constexpr int HALF = 128 * 128;      // one 64-dim half of a 128-row tile: 128 rows x 128 B
+constexpr int TILE = 2 * HALF;       // 128 rows x 128 dims bf16
+constexpr float RESCALE_LOG2 = 8.f;  // lazy-rescale threshold
+constexpr int EVERY_KEY = 0x3fffffff;
+
+template <int QT>
+struct Smem {
+  static constexpr int SLOTS = QT == 2 ? 5 : 2;  // ring of K_0, V_0, K_1, V_1, ...
+  uint8_t q[QT][TILE];
+  uint8_t kv[SLOTS][TILE];
+  uint64_t q_full, kv_full[SLOTS], kv_empty[SLOTS];
+  uint64_t s_full[QT], p_full[QT], o_full[QT];
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(Smem<2>) + 1024 <= 226 * 1024, "host requests 226 KB of dynamic shared memory (2 tiles)");
+static_assert(sizeof(Smem<1>) + 1024 <= 98 * 1024, "host requests 98 KB of dynamic shared memory (1 tile)");
+
+// What the body needs of a CTA's work: n key tiles, tile i starting at key
+// position key0(i); loads; and each row's visible keys
+// {kp : kp <= hi and (kp >= lo or kp < sinks)}.
+template <int QT, class Work>
+__device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, float scale_log2) {
+  constexpr int SLOTS = Smem<QT>::SLOTS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = w.n;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, 1);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&sm.kv_full[s], 1);
+      mbar_init(&sm.kv_empty[s], 1);
+    }
+    for (int t = 0; t < QT; ++t) {
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_full[t], 4);
+      mbar_init(&sm.o_full[t], 1);
+    }
+    sm.abort = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 4 * QT + 1) {
+    tmem_alloc(&sm.tmem, QT * 256);
+    tmem_relinquish();
+  }
+  w.clear_q(sm);
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();  // not before: a dependent's CTA must not take TMEM that this one has yet to allocate
+  const uint32_t tmem = sm.tmem;  // S_t at columns 128 t, O_t at 128 (QT + t)
+
+  if (warp == 4 * QT) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      w.load_q(sm, &sm.q_full);
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < n; ++i) {
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {
+          if (!mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
+            sm.abort = 1;
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&sm.kv_full[slot], TILE);
+          w.load_kv(sm.kv[slot], &sm.kv_full[slot], i, v);
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Drain: every copy has landed and been consumed before the CTA leaves.
+      for (int s = 0; ok && s < SLOTS; ++s) {
+        mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 4 * QT + 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t id_qk = idesc_bf16<128, 128>();
+      constexpr uint32_t id_pv = idesc_bf16<128, 128>() | (1u << 16);  // B (V) MN-major
+      int kslot = 0, vslot = 1 % SLOTS;
+      uint32_t kphase = 0, vphase = 0;
+      auto next = [](int& s, uint32_t& ph) {
+        s += 2;
+        if (s >= SLOTS) {
+          s -= SLOTS;
+          ph ^= 1;
+        }
+      };
+      auto qk = [&](int t) {
+        const uint32_t qb = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // K = 128 head dims, 16 per MMA
+          const uint32_t off = (k >> 2) * HALF + (k & 3) * 32;
+          mma_bf16(tmem + t * 128, sdesc_sw128(qb + off), sdesc_sw128(kb + off), id_qk, k > 0 ? 1u : 0u);
+        }
+        mma_commit(&sm.s_full[t]);
+      };
+      bool ok = mbar_wait(&sm.q_full, 0, FB_KERR_TIMEOUT_FULL) && mbar_wait(&sm.kv_full[0], 0, FB_KERR_TIMEOUT_FULL);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < QT; ++t) qk(t);
+        mma_commit(&sm.kv_empty[0]);
+        next(kslot, kphase);
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
+#pragma unroll 1
+        for (int t = 0; ok && t < QT; ++t) {
+          if (!mbar_wait(&sm.p_full[t], i & 1, FB_KERR_TIMEOUT_TMEM)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t vb = smem_u32(sm.kv[vslot]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)  // K = 128 keys, 16 per MMA
+            mma_bf16_ts(tmem + (QT + t) * 128, tmem + t * 128 + k * 8, sdesc_mn_sw128(vb + k * 2048, HALF, 1024),
+                        id_pv, (i > 0 || k > 0) ? 1u : 0u);
+          if (t == QT - 1) mma_commit(&sm.kv_empty[vslot]);
+          if (i + 1 < n) {
+            if (t == 0 && !mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            qk(t);
+          } else {
+            mma_commit(&sm.o_full[t]);
+          }
+        }
+        if (ok && i + 1 < n) {
+          mma_commit(&sm.kv_empty[kslot]);
+          next(kslot, kphase);
+        }
+        next(vslot, vphase);
+      }
+      if (!ok) sm.abort = 1;
+    }
+  } else {
+    // ---------------- softmax + epilogue ----------------
+    const int t = warp >> 2;                         // query tile
+    const int r = (warp & 3) * 32 + lane;            // row of the tile
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t * 128 + lane_base, t_o = tmem + (QT + t) * 128 + lane_base;
+    int hi, lo;
+    w.row_range(t, r, hi, lo);
+    const int sinks = w.sinks;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int k0 = w.key0(i);
+      if (!mbar_wait(&sm.s_full[t], i & 1, FB_KERR_TIMEOUT_TMEM)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sr[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) tmem_ld32(t_s + c, sr + c);
+      tmem_ld_wait();
+      // Edge tiles: scores of keys that the row does not see become -inf.
+      if (__any_sync(0xffffffffu, k0 + BK - 1 > hi || (k0 < lo && k0 + BK > sinks))) {
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          const int b = k0 + c;
+          const uint32_t seen = bits_below(hi + 1 - b) & (~bits_below(lo - b) | bits_below(sinks - b));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1u)) sr[c + e] = 0xff800000u;
+        }
+      }
+      if (t == 0 && w.zero_row(i, r)) {
+        // A key row behind the prompt's end holds another prompt's values or
+        // nothing at all, and 0 * NaN = NaN: its V row is zeroed once the copy
+        // has landed (tile 0's P V runs first, so once is enough).
+        const int slot = (2 * i + 1) % SLOTS;
+        if (!mbar_wait(&sm.kv_full[slot], ((2 * i + 1) / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
+        uint8_t* vrow = sm.kv[slot] + r * 128;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[c]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+      const float m_new = mx > m_run + RESCALE_LOG2 || m_run == -INFINITY ? fmaxf(m_run, mx) : m_run;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2f(m_run - m_use);  // 1 unless the max moved; 0 while nothing was seen
+      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(t_o + c, o);
+        }
+      }
+      float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 128; c += 64) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = exp2f(fmaf(__uint_as_float(sr[c + 2 * e]), scale_log2, -m_use));
+          const float p1 = exp2f(fmaf(__uint_as_float(sr[c + 2 * e + 1]), scale_log2, -m_use));
+          rs[(2 * e) & 3] += p0;
+          rs[(2 * e + 1) & 3] += p1;
+          const bf162 h = __floats2bfloat162_rn(p0, p1);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        tmem_st32(t_s + c / 2, pk);
+      }
+      tmem_st_wait();
+      l_run = l_run * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+      m_run = m_new;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[t]);
+    }
+    if (ok && mbar_wait(&sm.o_full[t], 0, FB_KERR_TIMEOUT_TMEM)) {
+      tc_fence_after();
+      w.store(t, r, t_o, m_run, l_run);
+    } else {
+      sm.abort = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 4 * QT + 1) tmem_dealloc(tmem, QT * 256);
+}
+
+template <int QT>
+__device__ __forceinline__ Smem<QT>& tile_smem() {
+  extern __shared__ uint8_t smem_raw[];
+  return *reinterpret_cast<Smem<QT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+}
+
+// ---- windowed causal prefill -----------------------------------------------------------
+// Key tiles of the query tile [qp0, qp0 + 128): those of the sinks, then those
+// of the window, at multiples of 128 of the prompt.
+template <int QT>
+struct WindowWork {
+  const CUtensorMap *tmQ, *tmK, *tmV;
+  bf16* out;
+  int ld_o, head0, kvh, s0, s1, qp0, window;
+  int n, n_sink, first, sinks;
+
+  __device__ __forceinline__ int key0(int i) const { return (i < n_sink ? i : i - n_sink + first) * BK; }
+  __device__ __forceinline__ bool zero_row(int i, int r) const { return key0(i) + r >= s1 - s0; }
+  __device__ __forceinline__ void clear_q(Smem<QT>&) const {}
+  __device__ __forceinline__ void load_q(Smem<QT>& sm, uint64_t* bar) const {
+    mbar_arrive_expect_tx(bar, QT * TILE);
+    for (int t = 0; t < QT; ++t)
+      for (int h = 0; h < 2; ++h) tma_load_2d(sm.q[t] + h * HALF, tmQ, bar, (head0 + t) * D + h * 64, s0 + qp0);
+  }
+  __device__ __forceinline__ void load_kv(uint8_t* dst, uint64_t* bar, int i, int v) const {
+    const int row = s0 + key0(i);
+    for (int h = 0; h < 2; ++h) tma_load_2d(dst + h * HALF, v ? tmV : tmK, bar, kvh * D + h * 64, row);
+  }
+  __device__ __forceinline__ void row_range(int, int r, int& hi, int& lo) const {
+    const int qpos = qp0 + r;
+    hi = s0 + qpos < s1 ? qpos : -1;
+    lo = qpos - window + 1;
+  }
+  __device__ __forceinline__ void store(int t, int r, uint32_t t_o, float, float l) const {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const bool live = s0 + qp0 + r < s1;
+    bf16* row = out + static_cast<size_t>(s0 + qp0 + r) * ld_o + (head0 + t) * D;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      tmem_ld32(t_o + c, o);
+      tmem_ld_wait();
+      if (live) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          float f[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[e + x]) * inv;
+          *reinterpret_cast<uint4*>(row + c + e) = pack8(f);
+        }
+      }
+    }
+  }
+};
+
+template <int QT>
+__device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV,
+                                               bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,
+                                               const int* tile_start, int Hq, int Hkv, int window, int sinks,
+                                               float scale_log2) {
+  pdl_wait();
+  WindowWork<QT> w;
+  w.tmQ = tmQ;
+  w.tmK = tmK;
+  w.tmV = tmV;
+  w.out = out;
+  w.ld_o = ld_o;
+  w.head0 = blockIdx.y * QT;  // QT heads of one KV head
+  w.kvh = w.head0 / (Hq / Hkv);
+  w.window = window;
+  const int seq = tile_seq[blockIdx.x];
+  w.s0 = cu_seqlens[seq];
+  w.s1 = cu_seqlens[seq + 1];
+  w.qp0 = tile_start[blockIdx.x];
+  const int end = min(w.qp0 + BQ, w.s1 - w.s0);  // queries and keys of this tile end here
+  if (w.qp0 < 0 || w.qp0 >= end) return;         // a tile table that does not match cu_seqlens
+  const int last = (end - 1) / BK;
+  w.sinks = min(sinks, end);
+  w.n_sink = min((w.sinks + BK - 1) / BK, last + 1);
+  w.first = max(max(w.qp0 - window + 1, 0) / BK, w.n_sink);
+  w.n = w.n_sink + last + 1 - w.first;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(tmQ);
+    tma_prefetch_desc(tmK);
+    tma_prefetch_desc(tmV);
+  }
+  tile_attention<QT>(w, tile_smem<QT>(), scale_log2);
+}
+
+// ---- shared prefix of a decode batch ---------------------------------------------------
+// items[blockIdx.x] = {first row, rows, first page, pages, part, 0, 0, 0}: the rows
+// (sequences) of one group against a range of the pages that its first row's
+// block table begins with. Row r of query tile t is head r / nb of the group's
+// KV head for sequence first + t * nb + r % nb, nb = 128 / G rounded down to a
+// multiple of 8 (whole swizzle atoms), so one TMA box of nb rows fetches one head.
+struct PrefixItem {
+  int row0, rows, page0, pages, part, pad[3];
+};
+
+template <int QT>
+struct PrefixWork {
+  const CUtensorMap *tmQ, *tmK, *tmV;
+  const int *pages, *seq_lens;
+  float *o_part, *ml_part;
+  PrefixItem it;
+  int kvh, G, nb, Hq, Hkv, parts, blocks;
+  int n, sinks;
+
+  __device__ __forceinline__ int key0(int i) const { return it.page0 * PAGE + i * BK; }
+  __device__ __forceinline__ bool zero_row(int, int) const { return false; }
+  // Rows that no head and sequence uses hold zeros and see every key: what
+  // they compute is finite and dropped, and keeps no warp on the masked path.
+  __device__ __forceinline__ void clear_q(Smem<QT>& sm) const {
+    const int rows = 128 - G * nb;
+    for (int e = threadIdx.x; e < QT * 2 * rows * 8; e += blockDim.x) {
+      const int half = e / (rows * 8);  // tile * 2 + dim half
+      *reinterpret_cast<uint4*>(sm.q[half >> 1] + (half & 1) * HALF + G * nb * 128 + (e % (rows * 8)) * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load_q(Smem<QT>& sm, uint64_t* bar) const {
+    mbar_arrive_expect_tx(bar, QT * 2 * G * nb * 128);
+    for (int t = 0; t < QT; ++t)
+      for (int g = 0; g < G; ++g)
+        for (int h = 0; h < 2; ++h)
+          tma_load_2d(sm.q[t] + h * HALF + g * nb * 128, tmQ, bar, (kvh * G + g) * D + h * 64, it.row0 + t * nb);
+  }
+  __device__ __forceinline__ void load_kv(uint8_t* dst, uint64_t* bar, int i, int v) const {
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+      // a tile's second page behind the end: rows past the cache, which TMA fills with zeros
+      int page = 2 * i + pg < it.pages ? pages[it.page0 + 2 * i + pg] : blocks;
+      if (page < 0 || page > blocks) {
+        set_status(FB_KERR_BAD_ARG);
+        page = blocks;
+      }
+      const int row = (page * Hkv + kvh) * PAGE;
+      for (int h = 0; h < 2; ++h)
+        tma_load_2d(dst + h * HALF + pg * PAGE * 128, v ? tmV : tmK, bar, h * 64, row);
+    }
+  }
+  __device__ __forceinline__ int row_of(int t, int r) const { return t * nb + r % nb; }  // of the item
+  __device__ __forceinline__ void row_range(int t, int r, int& hi, int& lo) const {
+    const int b = row_of(t, r);
+    const int end = (it.page0 + it.pages) * PAGE;
+    hi = r < G * nb && b < it.rows ? min(seq_lens[it.row0 + b], end) - 1 : EVERY_KEY;
+    lo = 0;
+  }
+  __device__ __forceinline__ void store(int t, int r, uint32_t t_o, float m, float l) const {
+    const int b = row_of(t, r);
+    const bool live = r < G * nb && b < it.rows;
+    const size_t at = (static_cast<size_t>(it.row0 + b) * Hq + kvh * G + r / nb) * parts + it.part;
+    if (live) *reinterpret_cast<float2*>(ml_part + 2 * at) = make_float2(m, l);
+    float* row = o_part + at * D;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      tmem_ld32(t_o + c, o);
+      tmem_ld_wait();
+      if (live) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<uint4*>(row + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      }
+    }
+  }
+};
+
+template <int QT>
+__device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const CUtensorMap* tmK,
+                                                 const CUtensorMap* tmV, const PrefixItem* items,
+                                                 const int* block_tables, int max_blocks, const int* seq_lens,
+                                                 float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts,
+                                                 int blocks, float scale_log2) {
+  pdl_wait();
+  PrefixWork<QT> w;
+  w.it = items[blockIdx.x];
+  if (w.it.pages <= 0) return;
+  w.tmQ = tmQ;
+  w.tmK = tmK;
+  w.tmV = tmV;
+  w.pages = block_tables + static_cast<size_t>(w.it.row0) * max_blocks;
+  w.seq_lens = seq_lens;
+  w.o_part = o_part;
+  w.ml_part = ml_part;
+  w.kvh = blockIdx.y;
+  w.G = G;
+  w.nb = (128 / G) & ~7;
+  w.Hq = Hq;
+  w.Hkv = Hkv;
+  w.parts = parts;
+  w.blocks = blocks;
+  w.n = (w.it.pages + 1) / 2;
+  w.sinks = 0;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(tmQ);
+    tma_prefetch_desc(tmK);
+    tma_prefetch_desc(tmV);
+  }
+  tile_attention<QT>(w, tile_smem<QT>(), scale_log2);
+}
+
+}  // namespace
+
+// q [T, Hq * 128] (tmQ), k, v [T, Hkv * 128] (tmK, tmV): tensor maps over the
+// packed rows, boxes of 64 dims x 128 rows, 128B swizzle. Grid: (query tiles
+// of tile_seq / tile_start, Hq / QT). out [T, ld_o] bf16, head h at columns
+// h * 128; rows outside every prompt are not written.
+#define FB_WINDOW_PREFILL(QT, CTAS)                                                                               \
+  extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_window_prefill_q##QT(                      \
+      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,                           \
+      const __grid_constant__ CUtensorMap tmV, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,   \
+      const int* tile_start, int Hq, int Hkv, int window, int sinks, float scale_log2) {                          \
+    window_prefill<QT>(&tmQ, &tmK, &tmV, out, ld_o, cu_seqlens, tile_seq, tile_start, Hq, Hkv, window, sinks,     \
+                       scale_log2);                                                                               \
+  }
+FB_WINDOW_PREFILL(1, 2)
+FB_WINDOW_PREFILL(2, 1)
+
+// q [B, Hq * 128] (tmQ, boxes of 64 dims x nb rows); caches viewed as [blocks *
+// Hkv * 64, 128] (tmK, tmV, boxes of 64 dims x one page). Grid: (items, Hkv).
+// Partial `part` of (row, head) at index (row * Hq + head) * parts + part.
+#define FB_PREFIX_ATTN(QT, CTAS)                                                                                  \
+  extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_prefix_attn_q##QT(                         \
+      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,                           \
+      const __grid_constant__ CUtensorMap tmV, const PrefixItem* items, const int* block_tables, int max_blocks,  \
+      const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts, int blocks,          \
+      float scale_log2) {                                                                                         \
+    prefix_attention<QT>(&tmQ, &tmK, &tmV, items, block_tables, max_blocks, seq_lens, o_part, ml_part, G, Hq, Hkv, \
+                         parts, blocks, scale_log2);                                                              \
+  }
+FB_PREFIX_ATTN(1, 2)
+FB_PREFIX_ATTN(2, 1)

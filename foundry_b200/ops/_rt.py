@@ -62,7 +62,8 @@ def function(image: str, name: str, smem: int = 0) -> int:
 # another kernel writes (csrc/kernels/fb_common.cuh). Kernels of other images
 # (the peer-memory collectives, MoE) launch in plain stream order. Set
 # FOUNDRY_PDL=0 to launch everything in plain order.
-PDL_IMAGES = frozenset({"elementwise", "attention", "attention_tc", "gemm_bf16"})
+PDL_IMAGES = frozenset({"elementwise", "attention", "attention_tc", "gemm_bf16", "attention_span", "attention_tile",
+                        "logprobs"})
 PDL_ENABLED = os.environ.get("FOUNDRY_PDL", "1") != "0"
 _pdl = threading.local()
 

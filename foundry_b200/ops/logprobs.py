@@ -1,0 +1,91 @@
+"""Log probabilities of given tokens, entropy and the most probable
+alternatives (csrc/kernels/logprobs.cu), beside the greedy ``argmax``."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _rt
+
+_IMG = "logprobs"
+MAX_TOP = 32
+CTAS_PER_SM = 4
+MIN_SHARE = 4096  # logits per CTA: below it the join of a row's pieces costs more than it saves
+_NAMES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+
+
+class LogprobWorkspace:
+    """Partial results of ``token_logprobs``, the same for every shape. Calls
+    that may run at the same time need a workspace each; calls in stream order,
+    captured graphs among them, may share one."""
+
+    def __init__(self, arena=None, device=None):
+        if arena is not None:
+            empty, zeros = arena.empty, arena.zeros
+        else:
+            device = device or torch.device("cuda", torch.cuda.current_device())
+            empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+            zeros = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+        self.ctas = CTAS_PER_SM * _rt.sm_count()
+        self.sums = empty((2 * self.ctas * 4,), torch.float32)
+        self.keys = empty((2 * self.ctas * MAX_TOP,), torch.int64)
+        self.tickets = zeros((self.ctas,), torch.int32)
+
+    def clear(self) -> None:
+        self.tickets.zero_()
+
+
+def _check(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def share_of(rows: int, vocab: int, ctas: int) -> int:
+    """Logits per CTA: an equal part of them all, in steps of 64."""
+    return max(MIN_SHARE, math.ceil(rows * vocab / ctas / 64) * 64)
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: torch.Tensor | None,
+                   entropy: torch.Tensor | None, top_logprobs: torch.Tensor | None = None,
+                   top_ids: torch.Tensor | None = None, *, ws: LogprobWorkspace) -> None:
+    """For each row of ``logits`` [T, V] (bf16, fp16 or fp32, any row stride):
+
+    ``logprobs`` [T] fp32      log softmax(row)[ids[row]]; 0 for a negative id (no token),
+                               NaN (and the image's status bit) for one past the vocabulary
+    ``entropy`` [T] fp32       -sum p ln p
+    ``top_logprobs`` [T, k] fp32, ``top_ids`` [T, k] int32: the k <= 32 most probable
+                               tokens, largest first, the lower token on ties
+
+    Outputs that are None are left out. Masked logits may be -inf or the
+    type's lowest value; a row that is -inf throughout, or holds +inf or NaN,
+    gives NaN (its ``top_ids`` are the order of its logits, NaN left out and -1
+    for what is missing)."""
+    _check(logits.dim() == 2 and logits.dtype in _NAMES and (logits.stride(1) == 1 or logits.shape[1] == 1),
+           "logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
+    t, v = logits.shape
+    _check(0 < v < 1 << 30, f"vocabulary of {v}")
+    k = 0
+    _check((top_logprobs is None) == (top_ids is None), "top_logprobs and top_ids come together")
+    if top_ids is not None:
+        k = top_ids.shape[-1]
+        _check(k <= min(MAX_TOP, v), f"at most {min(MAX_TOP, v)} alternatives, got {k}")
+    _check((ids is None) == (logprobs is None), "ids and logprobs come together")
+    cur = torch.cuda.current_device()
+    for x, dtype, shape in ((ids, torch.int32, (t,)), (logprobs, torch.float32, (t,)), (entropy, torch.float32, (t,)),
+                            (top_logprobs, torch.float32, (t, k)), (top_ids, torch.int32, (t, k)),
+                            (logits, logits.dtype, (t, v))):
+        if x is None:
+            continue
+        _check(x.dtype == dtype and tuple(x.shape) == shape, f"expected {dtype} {shape}, got {x.dtype} {tuple(x.shape)}")
+        _check(x is logits or x.is_contiguous(), "ids and outputs must be contiguous")
+        _check(x.is_cuda and x.get_device() == cur, f"tensors must be on the current CUDA device {cur}, got one on {x.device}")
+    if not t:
+        return
+    share = share_of(t, v, ws.ctas)
+    _rt.launch(_IMG, f"fb_logprobs_{_NAMES[logits.dtype]}", (min(ws.ctas, math.ceil(t * v / share)),), (256,), [
+        logits.data_ptr(), logits.stride(0), ids.data_ptr() if ids is not None else 0,
+        logprobs.data_ptr() if logprobs is not None else 0, entropy.data_ptr() if entropy is not None else 0,
+        top_logprobs.data_ptr() if k else 0, top_ids.data_ptr() if k else 0, ws.sums.data_ptr(), ws.keys.data_ptr(),
+        ws.tickets.data_ptr(), share, t, v, k])

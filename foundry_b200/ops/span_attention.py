@@ -1,0 +1,285 @@
+"""Attention over part of the context (csrc/kernels/attention_span.cu,
+attention_tile.cu): decode for a batch whose sequences share a long prompt,
+and a sliding window with sinks for decode and prefill. head_dim is 128, the
+KV page 64 tokens, tensors bf16, 1 to 16 query heads per KV head.
+
+Window and sinks: the query at position i sees key j iff ``j <= i`` and
+(``j > i - window`` or ``j < sinks``).
+
+A decode call is one launch (two with a shared prefix) that needs no plan of
+the lengths: it reads them on the device, so a captured graph stays valid as
+sequences grow.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .._native import core
+from . import _rt
+from .attention import LOG2E, PAGE, _rows_tmap
+
+_SPAN, _TILE = "attention_span", "attention_tile"
+MAX_GROUP = 16
+SPAN_SMEM = 74 * 1024
+TILE_SMEM = {1: 98 * 1024, 2: 226 * 1024}
+TILE = 128  # queries (and keys) of a tile
+_ITEM = 8  # int32 words of a prefix work item
+
+
+def _check(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def _check_device(*tensors: torch.Tensor) -> None:
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        _check(t.is_cuda and t.get_device() == cur,
+               f"tensors must be on the current CUDA device {cur}, got one on {t.device}")
+
+
+def _check_scale(scale: float | None) -> float:
+    if scale is None:
+        return 1.0 / math.sqrt(128)
+    _check(math.isfinite(scale) and scale > 0, f"scale must be positive, got {scale}")
+    return float(scale)
+
+
+def _check_window(window: int, sinks: int) -> None:
+    _check(0 < window < 1 << 30 and 0 <= sinks < 1 << 30, f"window must be at least 1 and sinks at least 0, got {window}, {sinks}")
+
+
+def _check_group(n_q: int, n_kv: int) -> int:
+    _check(n_kv > 0 and n_q % n_kv == 0 and 1 <= n_q // n_kv <= MAX_GROUP,
+           f"{n_q} query heads for {n_kv} KV heads: a whole number from 1 to {MAX_GROUP} per KV head")
+    return n_q // n_kv
+
+
+def _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int, int, int, int, int]:
+    """(batch, n_q, n_kv, blocks, max_blocks) of a decode call."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    _check(q.dim() == 3 and q.shape[2] == 128 and q.dtype == bf16, "q must be bf16 [batch, heads, 128]")
+    b, n_q, _ = q.shape
+    _check(out.shape == q.shape and out.dtype == bf16, "out must be bf16 of q's shape")
+    for t in (q, out):
+        _check(t.stride(2) == 1 and t.stride(1) == 128 and (t.stride(0) % 8 == 0 or b == 1) and t.data_ptr() % 16 == 0,
+               "q and out must hold a row's heads next to each other, rows at multiples of 16 bytes")
+    _check(b <= 1 or out.stride(0) >= n_q * 128, "out's rows overlap")
+    _check(k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (PAGE, 128) and k_cache.shape == v_cache.shape
+           and k_cache.dtype == bf16 and v_cache.dtype == bf16, f"caches must be bf16 [blocks, kv heads, {PAGE}, 128]")
+    _check(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+    blocks, n_kv = k_cache.shape[:2]
+    _check(blocks > 0 and (blocks + 1) * n_kv * PAGE < 1 << 31, "cache of no or too many blocks")
+    _check(block_tables.dtype == i32 and block_tables.dim() == 2 and block_tables.shape[0] == b
+           and block_tables.is_contiguous(), "block_tables must be contiguous int32 [batch, max_blocks]")
+    _check(seq_lens.dtype == i32 and tuple(seq_lens.shape) == (b,) and seq_lens.is_contiguous(),
+           "seq_lens must be contiguous int32 [batch]")
+    max_blocks = block_tables.shape[1]
+    _check(0 < max_blocks and b * n_kv * (max_blocks // 2 + 2) < 1 << 31, "block_tables of no or too many pages")
+    _check_device(q, k_cache, v_cache, block_tables, seq_lens, out)
+    return b, n_q, n_kv, blocks, max_blocks
+
+
+def _page_tmap(cache: torch.Tensor, box_rows: int) -> bytes:
+    """TMA map of a paged cache [blocks, Hkv, 64, 128] viewed as [rows, 128]:
+    64-column x ``box_rows`` boxes, 128B swizzle."""
+    rows = cache.shape[0] * cache.shape[1] * PAGE
+    return core().make_tmap_2d(cache.data_ptr(), 9, 128, rows, 256, 64, box_rows, 3)
+
+
+def span_grid(group: int) -> int:
+    """CTAs of a decode launch: all that are resident at once."""
+    return _rt.sm_count() * (3 if group <= 8 else 2)
+
+
+class SpanWorkspace:
+    """Partial results of the decode calls: two pieces per CTA (the same for
+    every batch and length), and ``partials`` (row, head, part) results of
+    shared prefixes (``PrefixPlan.partials``; 0 if there are none). With
+    ``arena`` the buffers come from it (a runner whose graphs are saved).
+
+    Calls that may run at the same time need a workspace each; calls in stream
+    order, captured graphs among them, may share one. Every call leaves
+    ``tickets`` zeroed; ``clear()`` puts that right after a device-side error."""
+
+    def __init__(self, partials: int = 0, arena=None, device=None):
+        if arena is not None:
+            empty, zeros = arena.empty, arena.zeros
+        else:
+            device = device or torch.device("cuda", torch.cuda.current_device())
+            empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+            zeros = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+        self.ctas = 3 * _rt.sm_count()
+        pieces = max(2 * self.ctas * 8, 2 * span_grid(MAX_GROUP) * MAX_GROUP)  # (piece, head) pairs
+        self.o = empty((pieces * 128,), torch.float32)
+        self.ml = empty((pieces * 2,), torch.float32)
+        self.tickets = zeros((self.ctas,), torch.int32)
+        self.partials = partials
+        self.prefix_o = empty((max(partials, 1) * 128,), torch.float32)
+        self.prefix_ml = empty((max(partials, 1) * 2,), torch.float32)
+
+    def clear(self) -> None:
+        self.tickets.zero_()
+
+
+def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, dims, window: int, sinks: int,
+          scale: float, plan: "PrefixPlan | None") -> None:
+    b, n_q, n_kv, blocks, max_blocks = dims
+    g = n_q // n_kv
+    grid = min(span_grid(g), ws.ctas, b * n_kv * (max_blocks // 2 + 2))
+    _rt.launch(_SPAN, f"fb_span_attn_g{4 if g <= 4 else 8 if g <= 8 else 16}", (grid,), (192,), [
+        _page_tmap(k_cache, PAGE), _page_tmap(v_cache, PAGE), _page_tmap(k_cache, 16), _page_tmap(v_cache, 16),
+        q.data_ptr(), q.stride(0), block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(),
+        out.stride(0), b, n_kv, g, window, sinks, plan.row_info.data_ptr() if plan else 0, ws.prefix_o.data_ptr(),
+        ws.prefix_ml.data_ptr(), plan.parts if plan else 0, ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(),
+        float(scale * LOG2E)], smem=SPAN_SMEM)
+
+
+def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, out: torch.Tensor, window: int, sinks: int, ws: SpanWorkspace,
+                            scale: float | None = None) -> torch.Tensor:
+    """Decode attention over the last ``window`` tokens (the current one among
+    them) and the first ``sinks`` ones. Arguments as for ``decode_attention``;
+    q and out [B, Hq, 128] may have any row stride that is a multiple of 8.
+
+    Block-table entries of pages without a visible token are never read: their
+    pages may have been freed. Rows of length 0 get zeros."""
+    dims = _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out)
+    _check_group(dims[1], dims[2])
+    _check_window(window, sinks)
+    scale = _check_scale(scale)
+    if dims[0]:
+        _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, window, sinks, scale, None)
+    return out
+
+
+def prefix_rows(group: int) -> int:
+    """Sequences of a 128-row query tile: whole groups of 8 rows per head."""
+    return (128 // group) & ~7
+
+
+def _prefix_splits(tiles: int, pages: int, slots: int) -> int:
+    """Parts that the ``pages`` of a prefix are cut into, ``tiles`` CTAs each:
+    the cut with the shortest schedule of ``slots`` CTAs at a time, where a
+    part costs its key tiles and about three more for its start and its end."""
+    keys = math.ceil(pages / 2)
+    best = min((math.ceil(tiles * s / slots) * (math.ceil(keys / s) + 3), s) for s in range(1, min(keys, 64) + 1))
+    return best[1]
+
+
+class PrefixPlan:
+    """Which rows of a decode batch share how many leading pages.
+
+    Group g holds the next ``group_sizes[g]`` rows; the first
+    ``prefix_pages[g]`` entries of their block tables are the same pages
+    (0: nothing shared). The lengths need not be known, only that; a row may
+    even be shorter than its prefix (a padding row of length 0). The plan
+    holds until the batch's composition changes: captured graphs read it, so
+    it has to outlive them."""
+
+    def __init__(self, group_sizes: list[int], prefix_pages: list[int], n_q: int, n_kv: int, max_blocks: int,
+                 arena=None, device=None):
+        group = _check_group(n_q, n_kv)
+        _check(len(group_sizes) == len(prefix_pages), "one number of prefix pages for each group")
+        _check(all(n >= 0 for n in group_sizes) and all(0 <= p <= max_blocks for p in prefix_pages),
+               f"group sizes must not be negative, prefixes 0 to {max_blocks} pages")
+        self.n_q, self.n_kv, self.max_blocks = n_q, n_kv, max_blocks
+        self.rows = sum(group_sizes)
+        nb = prefix_rows(group)
+        shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n and p]
+        # two query tiles per CTA as soon as a group has more rows than one
+        self.tiles = 2 if any(n > nb for n, _ in shared) else 1
+        step = nb * self.tiles
+        slots = max(1, _rt.sm_count() * (1 if self.tiles == 2 else 2) // n_kv)
+        ctas = sum(math.ceil(n / step) for n, _ in shared)
+        items, info, row, self.parts = [], [], 0, 0
+        for n, pages in zip(group_sizes, prefix_pages):
+            parts = 0
+            if n and pages:
+                splits = _prefix_splits(ctas, pages, slots)
+                keys = math.ceil(pages / 2)
+                cuts = [2 * (keys * s // splits) for s in range(splits)] + [pages]
+                parts = splits
+                for r0 in range(0, n, step):
+                    items += [[row + r0, min(step, n - r0), a, e - a, p, 0, 0, 0]
+                              for p, (a, e) in enumerate(zip(cuts, cuts[1:]))]
+            info += [[pages * PAGE if parts else 0, parts]] * n
+            self.parts = max(self.parts, parts)
+            row += n
+        self.items_n = len(items)
+        self.partials = self.rows * n_q * self.parts  # (row, head, part) results that a SpanWorkspace has to hold
+        host = torch.tensor(items or [[0] * _ITEM], dtype=torch.int32), torch.tensor(info or [[0, 0]], dtype=torch.int32)
+        if arena is not None:
+            self.items, self.row_info = (arena.empty(tuple(t.shape), torch.int32) for t in host)
+            self.items.copy_(host[0])
+            self.row_info.copy_(host[1])
+        else:
+            device = device or torch.device("cuda", torch.cuda.current_device())
+            self.items, self.row_info = (t.to(device) for t in host)
+
+
+def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, out: torch.Tensor, plan: PrefixPlan, ws: SpanWorkspace,
+                            scale: float | None = None) -> torch.Tensor:
+    """Decode attention for a batch whose rows share leading pages by groups
+    (``plan``): each group's shared pages are read once, for all its rows. The
+    result and the arguments are those of ``decode_attention`` (``seq_lens``
+    counts all tokens, ``block_tables`` begin with the shared pages). Rows of
+    length 0 get zeros."""
+    dims = _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out)
+    b, n_q, n_kv, blocks, max_blocks = dims
+    _check((plan.rows, plan.n_q, plan.n_kv, plan.max_blocks) == (b, n_q, n_kv, max_blocks),
+           f"plan for {plan.rows} rows, {plan.n_q} / {plan.n_kv} heads and {plan.max_blocks} pages, "
+           f"got {b}, {n_q} / {n_kv} and {max_blocks}")
+    _check(plan.partials <= ws.partials, f"workspace of {ws.partials} partial results, {plan.partials} needed")
+    _check_device(plan.items)
+    scale = _check_scale(scale)
+    if not b:
+        return out
+    if plan.items_n:
+        g = n_q // n_kv
+        q_map = core().make_tmap_2d(q.data_ptr(), 9, n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, 64,
+                                    prefix_rows(g), 3)
+        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (128 * plan.tiles + 64,), [
+            q_map, _page_tmap(k_cache, PAGE), _page_tmap(v_cache, PAGE), plan.items.data_ptr(),
+            block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(),
+            g, n_q, n_kv, plan.parts, blocks, float(scale * LOG2E)], smem=TILE_SMEM[plan.tiles])
+    _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan)
+    return out
+
+
+def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             cu_seqlens: torch.Tensor, tile_seq: torch.Tensor, tile_start: torch.Tensor,
+                             n_q: int, n_kv: int, window: int, sinks: int,
+                             scale: float | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts with a sliding window and sinks.
+    q: [T, *] with head h at columns h * 128 (row stride q.stride(0)); k, v
+    likewise with n_kv heads; out [T, n_q * 128]. The tile tables come from
+    ``prefill_tiles(seqlens)``. Rows outside every prompt are neither used
+    (they may hold anything) nor written."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    group = _check_group(n_q, n_kv)
+    _check_window(window, sinks)
+    scale = _check_scale(scale)
+    for t, heads, name in ((q, n_q, "q"), (k, n_kv, "k"), (v, n_kv, "v"), (out, n_q, "out")):
+        _check(t.dim() == 2 and t.dtype == bf16 and t.shape[1] >= heads * 128, f"{name} must be bf16 [T, >= {heads} * 128]")
+        _check(t.shape[0] == q.shape[0], f"{name} has {t.shape[0]} rows, q has {q.shape[0]}")
+    t = q.shape[0]
+    _check(out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0
+           and (t <= 1 or out.stride(0) >= n_q * 128), "out must be row-contiguous with 16-byte aligned rows")
+    for x in (cu_seqlens, tile_seq, tile_start):
+        _check(x.dtype == i32 and x.dim() == 1 and x.is_contiguous(), "cu_seqlens and the tile tables must be contiguous int32")
+    _check(tile_seq.numel() == tile_start.numel() and cu_seqlens.numel() >= 1, "tile tables of different lengths")
+    _check_device(q, k, v, out, cu_seqlens, tile_seq, tile_start)
+    n_tiles = tile_seq.numel()
+    if not n_tiles or not t:
+        return out
+    qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
+    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (n_tiles, n_q // qt), (128 * qt + 64,), [
+        _rows_tmap(q[:, : n_q * 128]), _rows_tmap(k[:, : n_kv * 128]), _rows_tmap(v[:, : n_kv * 128]),
+        out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(), tile_start.data_ptr(), n_q, n_kv,
+        window, sinks, float(scale * LOG2E)], smem=TILE_SMEM[qt])
+    return out
