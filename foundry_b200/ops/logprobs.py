@@ -11,7 +11,8 @@ from . import _rt
 
 _IMG = "logprobs"
 MAX_TOP = 32
-CTAS_PER_SM = 4
+CTAS_PER_SM = 3
+SMEM = 75 * 1024
 MIN_SHARE = 4096  # logits per CTA: below it the join of a row's pieces costs more than it saves
 _NAMES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
 
@@ -42,9 +43,15 @@ def _check(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def share_of(rows: int, vocab: int, ctas: int) -> int:
-    """Logits per CTA: an equal part of them all, in steps of 64."""
-    return max(MIN_SHARE, math.ceil(rows * vocab / ctas / 64) * 64)
+def share_of(rows: int, vocab: int, ctas: int) -> tuple[int, int]:
+    """(logits per CTA, flat distance of two rows). Up to ``ctas`` rows, each
+    has a whole number of CTAs of its own; more rows are one flat sequence cut
+    into equal shares."""
+    if rows <= ctas:
+        parts = max(1, min(ctas // rows, vocab // MIN_SHARE))
+        share = math.ceil(vocab / parts / 64) * 64
+        return share, math.ceil(vocab / share) * share
+    return math.ceil(rows * vocab / ctas / 64) * 64, vocab
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: torch.Tensor | None,
@@ -83,9 +90,9 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
         _check(x.is_cuda and x.get_device() == cur, f"tensors must be on the current CUDA device {cur}, got one on {x.device}")
     if not t:
         return
-    share = share_of(t, v, ws.ctas)
-    _rt.launch(_IMG, f"fb_logprobs_{_NAMES[logits.dtype]}", (min(ws.ctas, math.ceil(t * v / share)),), (256,), [
+    share, pitch = share_of(t, v, ws.ctas)
+    _rt.launch(_IMG, f"fb_logprobs_{_NAMES[logits.dtype]}", (min(ws.ctas, math.ceil(t * pitch / share)),), (256,), [
         logits.data_ptr(), logits.stride(0), ids.data_ptr() if ids is not None else 0,
         logprobs.data_ptr() if logprobs is not None else 0, entropy.data_ptr() if entropy is not None else 0,
         top_logprobs.data_ptr() if k else 0, top_ids.data_ptr() if k else 0, ws.sums.data_ptr(), ws.keys.data_ptr(),
-        ws.tickets.data_ptr(), share, t, v, k])
+        ws.tickets.data_ptr(), share, pitch, t, v, k], smem=SMEM)

@@ -48,7 +48,7 @@ def _check(x, ids, k, ws=None):
     ref = y - z.log()
     p = ref.exp()
     far = torch.where(p > 0, -y, 0.0)
-    share = min(v, L.share_of(t, v, L.CTAS_PER_SM * torch.cuda.get_device_properties(0).multi_processor_count))
+    share = min(v, L.share_of(t, v, L.CTAS_PER_SM * torch.cuda.get_device_properties(0).multi_processor_count)[0])
     rel = (share / 256 + 16 + 24) * 2.0**-24 + 2.0**-22 + (p * far).sum(-1) * 2.0**-23
     at = ids.long().clamp_min(0)
     want = ref.gather(1, at[:, None])[:, 0]
