@@ -8,6 +8,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <array>
 #include <chrono>
 #include <fstream>
 #include <mutex>
@@ -194,6 +195,27 @@ py::bytes rt_make_tmap_3d(uint64_t ptr, int dtype, uint64_t d0, uint64_t d1, uin
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
             "cuTensorMapEncodeTiled");
   return py::bytes(reinterpret_cast<const char*>(&m), sizeof(m));
+}
+
+// 2-D bf16 tensor maps with 64-column x box_rows boxes and the 128-byte swizzle,
+// one after another in one byte string (a kernel that needs several takes them
+// as one struct): (address, columns, rows, row stride in bytes, box rows) each.
+py::bytes rt_make_tmaps_bf16(const std::vector<std::array<uint64_t, 5>>& maps) {
+  std::vector<CUtensorMap> m(maps.size());
+  for (size_t i = 0; i < maps.size(); ++i) {
+    const auto& a = maps[i];
+    cuuint64_t dims[2] = {a[1], a[2]};
+    cuuint64_t strides[1] = {a[3]};
+    cuuint32_t box[2] = {64, static_cast<cuuint32_t>(a[4])};
+    cuuint32_t estr[2] = {1, 1};
+    check_drv(fb_driver()->cuTensorMapEncodeTiled(&m[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                                  reinterpret_cast<void*>(a[0]), dims, strides, box, estr,
+                                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+              "cuTensorMapEncodeTiled");
+  }
+  return py::bytes(reinterpret_cast<const char*>(m.data()), m.size() * sizeof(CUtensorMap));
 }
 
 // Address of a __device__ global of an image (e.g. an error-status word).
@@ -418,6 +440,7 @@ PYBIND11_MODULE(_C, m) {
         py::arg("row_stride_bytes"), py::arg("box_inner"), py::arg("box_outer"), py::arg("swizzle"),
         py::arg("l2promo") = 2);
   m.def("make_tmap_3d", &rt_make_tmap_3d);
+  m.def("make_tmaps_bf16", &rt_make_tmaps_bf16);
   m.def("get_global", &rt_get_global);
   m.def("func_attr", &rt_func_attr);
   m.def("func_num_params", [](uintptr_t fn) { return func_info(reinterpret_cast<CUfunction>(fn)).params.size(); });

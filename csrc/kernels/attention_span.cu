@@ -507,19 +507,22 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
 
 }  // namespace
 
-// Caches viewed as [blocks * Hkv * 64, 128]: tmK, tmV with boxes of a page x 64
-// dims, tmK16, tmV16 of 16 rows x 64 dims, 128B swizzle.
+// Caches viewed as [blocks * Hkv * 64, 128], K and V with boxes of a page x 64
+// dims, then K and V with boxes of 16 rows x 64 dims, 128B swizzle.
+struct SpanMaps {
+  CUtensorMap k, v, k16, v16;
+};
+
 #define FB_SPAN_INSTANCE(GP, CTAS)                                                                                \
   extern "C" __global__ void __launch_bounds__(THREADS, CTAS) fb_span_attn_g##GP(                                 \
-      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,                           \
-      const __grid_constant__ CUtensorMap tmK16, const __grid_constant__ CUtensorMap tmV16, const bf16* q,        \
-      long long ld_q, const int* block_tables, int max_blocks, int blocks, const int* seq_lens, bf16* out,        \
-      long long ld_o, int B, int Hkv, int G, int window, int sinks, const int2* row_info, const float* prefix_o,  \
-      const float* prefix_ml, int prefix_parts, float* ws_o, float* ws_ml, int* tickets, float scale_log2) {      \
+      const __grid_constant__ SpanMaps maps, const bf16* q, long long ld_q, const int* block_tables,              \
+      int max_blocks, int blocks, const int* seq_lens, bf16* out, long long ld_o, int B, int Hkv, int G,          \
+      int window, int sinks, const int2* row_info, const float* prefix_o, const float* prefix_ml,                 \
+      int prefix_parts, float* ws_o, float* ws_ml, int* tickets, float scale_log2) {                              \
     const Params a{q,     block_tables, seq_lens, row_info, out, prefix_o, prefix_ml,    ws_o,   ws_ml, tickets,  \
                    ld_q,  ld_o,         max_blocks, blocks, B,   Hkv,      G,            prefix_parts, window,    \
                    sinks, scale_log2};                                                                            \
-    span_body<GP>(&tmK, &tmV, &tmK16, &tmV16, a);                                                                 \
+    span_body<GP>(&maps.k, &maps.v, &maps.k16, &maps.v16, a);                                                     \
   }
 
 FB_SPAN_INSTANCE(4, 3)

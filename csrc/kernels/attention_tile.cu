@@ -499,32 +499,34 @@ __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const C
 
 }  // namespace
 
-// q [T, Hq * 128] (tmQ), k, v [T, Hkv * 128] (tmK, tmV): tensor maps over the
-// packed rows, boxes of 64 dims x 128 rows, 128B swizzle. Grid: (query tiles
-// of tile_seq / tile_start, Hq / QT). out [T, ld_o] bf16, head h at columns
-// h * 128; rows outside every prompt are not written.
+// Boxes of 64 dims, 128B swizzle: of q, then of k and v.
+struct TileMaps {
+  CUtensorMap q, k, v;
+};
+
+// q [T, Hq * 128], k, v [T, Hkv * 128]: maps over the packed rows, boxes of 128
+// rows. Grid: (query tiles of tile_seq / tile_start, Hq / QT). out [T, ld_o]
+// bf16, head h at columns h * 128; rows outside every prompt are not written.
 #define FB_WINDOW_PREFILL(QT, CTAS)                                                                               \
   extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_window_prefill_q##QT(                      \
-      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,                           \
-      const __grid_constant__ CUtensorMap tmV, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,   \
+      const __grid_constant__ TileMaps maps, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,     \
       const int* tile_start, int Hq, int Hkv, int window, int sinks, float scale_log2) {                          \
-    window_prefill<QT>(&tmQ, &tmK, &tmV, out, ld_o, cu_seqlens, tile_seq, tile_start, Hq, Hkv, window, sinks,     \
-                       scale_log2);                                                                               \
+    window_prefill<QT>(&maps.q, &maps.k, &maps.v, out, ld_o, cu_seqlens, tile_seq, tile_start, Hq, Hkv, window,   \
+                       sinks, scale_log2);                                                                        \
   }
 FB_WINDOW_PREFILL(1, 2)
 FB_WINDOW_PREFILL(2, 1)
 
-// q [B, Hq * 128] (tmQ, boxes of 64 dims x nb rows); caches viewed as [blocks *
-// Hkv * 64, 128] (tmK, tmV, boxes of 64 dims x one page). Grid: (items, Hkv).
-// Partial `part` of (row, head) at index (row * Hq + head) * parts + part.
+// q [B, Hq * 128] with boxes of nb rows; caches viewed as [blocks * Hkv * 64,
+// 128] with boxes of one page. Grid: (items, Hkv). Partial `part` of (row, head)
+// at index (row * Hq + head) * parts + part.
 #define FB_PREFIX_ATTN(QT, CTAS)                                                                                  \
   extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_prefix_attn_q##QT(                         \
-      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,                           \
-      const __grid_constant__ CUtensorMap tmV, const PrefixItem* items, const int* block_tables, int max_blocks,  \
+      const __grid_constant__ TileMaps maps, const PrefixItem* items, const int* block_tables, int max_blocks,    \
       const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts, int blocks,          \
       float scale_log2) {                                                                                         \
-    prefix_attention<QT>(&tmQ, &tmK, &tmV, items, block_tables, max_blocks, seq_lens, o_part, ml_part, G, Hq, Hkv, \
-                         parts, blocks, scale_log2);                                                              \
+    prefix_attention<QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \
+                         G, Hq, Hkv, parts, blocks, scale_log2);                                                  \
   }
 FB_PREFIX_ATTN(1, 2)
 FB_PREFIX_ATTN(2, 1)

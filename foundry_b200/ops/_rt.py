@@ -93,6 +93,11 @@ def launch(image: str, name: str, grid, block, args, smem: int = 0, stream: int 
                   pdl_active() and image in PDL_IMAGES)
 
 
+def raw_stream() -> int:
+    """The current stream's handle, without the Stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def status(image: str) -> int:
     """The image's device status word (0 = healthy; bits = bounded-wait timeouts)."""
     ptr, _ = core().get_global(image_hash(image), "fb_status")

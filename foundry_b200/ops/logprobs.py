@@ -14,7 +14,7 @@ MAX_TOP = 32
 CTAS_PER_SM = 3
 SMEM = 75 * 1024
 MIN_SHARE = 4096  # logits per CTA: below it the join of a row's pieces costs more than it saves
-_NAMES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_NAMES = {torch.bfloat16: "fb_logprobs_bf16", torch.float16: "fb_logprobs_f16", torch.float32: "fb_logprobs_f32"}
 
 
 class LogprobWorkspace:
@@ -36,11 +36,6 @@ class LogprobWorkspace:
 
     def clear(self) -> None:
         self.tickets.zero_()
-
-
-def _check(cond: bool, what: str) -> None:
-    if not cond:
-        raise ValueError(what)
 
 
 def share_of(rows: int, vocab: int, ctas: int) -> tuple[int, int]:
@@ -69,30 +64,33 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
     type's lowest value; a row that is -inf throughout, or holds +inf or NaN,
     gives NaN (its ``top_ids`` are the order of its logits, NaN left out and -1
     for what is missing)."""
-    _check(logits.dim() == 2 and logits.dtype in _NAMES and (logits.stride(1) == 1 or logits.shape[1] == 1),
-           "logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
+    if logits.dim() != 2 or logits.dtype not in _NAMES or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise ValueError("logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
     t, v = logits.shape
-    _check(0 < v < 1 << 30, f"vocabulary of {v}")
+    if not 0 < v < 1 << 30:
+        raise ValueError(f"vocabulary of {v}")
+    if (top_logprobs is None) != (top_ids is None) or (ids is None) != (logprobs is None):
+        raise ValueError("top_logprobs and top_ids come together, and ids and logprobs")
     k = 0
-    _check((top_logprobs is None) == (top_ids is None), "top_logprobs and top_ids come together")
     if top_ids is not None:
         k = top_ids.shape[-1]
-        _check(k <= min(MAX_TOP, v), f"at most {min(MAX_TOP, v)} alternatives, got {k}")
-    _check((ids is None) == (logprobs is None), "ids and logprobs come together")
+        if k > min(MAX_TOP, v):
+            raise ValueError(f"at most {min(MAX_TOP, v)} alternatives, got {k}")
     cur = torch.cuda.current_device()
+    if logits.get_device() != cur or ws.tickets.get_device() != cur:
+        raise ValueError(f"logits and workspace must be on the current CUDA device {cur}")
+    ptrs = []
     for x, dtype, shape in ((ids, torch.int32, (t,)), (logprobs, torch.float32, (t,)), (entropy, torch.float32, (t,)),
-                            (top_logprobs, torch.float32, (t, k)), (top_ids, torch.int32, (t, k)),
-                            (logits, logits.dtype, (t, v))):
+                            (top_logprobs, torch.float32, (t, k)), (top_ids, torch.int32, (t, k))):
         if x is None:
+            ptrs.append(0)
             continue
-        _check(x.dtype == dtype and tuple(x.shape) == shape, f"expected {dtype} {shape}, got {x.dtype} {tuple(x.shape)}")
-        _check(x is logits or x.is_contiguous(), "ids and outputs must be contiguous")
-        _check(x.is_cuda and x.get_device() == cur, f"tensors must be on the current CUDA device {cur}, got one on {x.device}")
+        if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.get_device() != cur:
+            raise ValueError(f"expected contiguous {dtype} {shape} on device {cur}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        ptrs.append(x.data_ptr())
     if not t:
         return
     share, pitch = share_of(t, v, ws.ctas)
-    _rt.launch(_IMG, f"fb_logprobs_{_NAMES[logits.dtype]}", (min(ws.ctas, math.ceil(t * pitch / share)),), (256,), [
-        logits.data_ptr(), logits.stride(0), ids.data_ptr() if ids is not None else 0,
-        logprobs.data_ptr() if logprobs is not None else 0, entropy.data_ptr() if entropy is not None else 0,
-        top_logprobs.data_ptr() if k else 0, top_ids.data_ptr() if k else 0, ws.sums.data_ptr(), ws.keys.data_ptr(),
-        ws.tickets.data_ptr(), share, pitch, t, v, k], smem=SMEM)
+    _rt.launch(_IMG, _NAMES[logits.dtype], (min(ws.ctas, math.ceil(t * pitch / share)),), (256,), [
+        logits.data_ptr(), logits.stride(0), *ptrs, ws.sums.data_ptr(), ws.keys.data_ptr(), ws.tickets.data_ptr(),
+        share, pitch, t, v, k], SMEM, _rt.raw_stream())

@@ -19,7 +19,7 @@ import torch
 
 from .._native import core
 from . import _rt
-from .attention import LOG2E, PAGE, _rows_tmap
+from .attention import LOG2E, PAGE
 
 _SPAN, _TILE = "attention_span", "attention_tile"
 MAX_GROUP = 16
@@ -27,6 +27,7 @@ SPAN_SMEM = 74 * 1024
 TILE_SMEM = {1: 98 * 1024, 2: 226 * 1024}
 TILE = 128  # queries (and keys) of a tile
 _ITEM = 8  # int32 words of a prefix work item
+_BF16, _I32 = torch.bfloat16, torch.int32
 
 
 def _check(cond: bool, what: str) -> None:
@@ -34,48 +35,70 @@ def _check(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _check_device(*tensors: torch.Tensor) -> None:
+def _check_device(*tensors: torch.Tensor) -> int:
     cur = torch.cuda.current_device()
     for t in tensors:
-        _check(t.is_cuda and t.get_device() == cur,
-               f"tensors must be on the current CUDA device {cur}, got one on {t.device}")
+        if t.get_device() != cur:
+            raise ValueError(f"tensors must be on the current CUDA device {cur}, got one on {t.device}")
+    return cur
 
 
 def _check_scale(scale: float | None) -> float:
     if scale is None:
         return 1.0 / math.sqrt(128)
-    _check(math.isfinite(scale) and scale > 0, f"scale must be positive, got {scale}")
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale must be positive, got {scale}")
     return float(scale)
 
 
 def _check_window(window: int, sinks: int) -> None:
-    _check(0 < window < 1 << 30 and 0 <= sinks < 1 << 30, f"window must be at least 1 and sinks at least 0, got {window}, {sinks}")
+    if not (0 < window < 1 << 30 and 0 <= sinks < 1 << 30):
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window}, {sinks}")
 
 
 def _check_group(n_q: int, n_kv: int) -> int:
-    _check(n_kv > 0 and n_q % n_kv == 0 and 1 <= n_q // n_kv <= MAX_GROUP,
-           f"{n_q} query heads for {n_kv} KV heads: a whole number from 1 to {MAX_GROUP} per KV head")
+    if not (n_kv > 0 and n_q % n_kv == 0 and 1 <= n_q // n_kv <= MAX_GROUP):
+        raise ValueError(f"{n_q} query heads for {n_kv} KV heads: a whole number from 1 to {MAX_GROUP} per KV head")
     return n_q // n_kv
 
 
-def _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int, int, int, int, int]:
-    """(batch, n_q, n_kv, blocks, max_blocks) of a decode call."""
-    bf16, i32 = torch.bfloat16, torch.int32
-    _check(q.dim() == 3 and q.shape[2] == 128 and q.dtype == bf16, "q must be bf16 [batch, heads, 128]")
+def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int, int, int, int, int]:
+    """(batch, n_q, n_kv, blocks, max_blocks) of a decode call, or a ValueError."""
+    if q.dim() == 3 and k_cache.dim() == 4 and block_tables.dim() == 2:
+        # What almost every call is, seen with few questions; anything else is looked at one by one.
+        b, n_q, d = q.shape
+        blocks, n_kv, page, _ = shape = k_cache.shape
+        max_blocks = block_tables.shape[1]
+        cur = torch.cuda.current_device()
+        if (d == 128 and page == PAGE and shape[3] == 128 and q.dtype is _BF16 and k_cache.dtype is _BF16
+                and v_cache.dtype is _BF16 and out.dtype is _BF16 and block_tables.dtype is _I32
+                and seq_lens.dtype is _I32 and out.shape == q.shape and v_cache.shape == shape
+                and block_tables.shape[0] == b and seq_lens.shape == (b,) and q.is_contiguous()
+                and out.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+                and block_tables.is_contiguous() and seq_lens.is_contiguous() and q.get_device() == cur
+                and k_cache.get_device() == cur and v_cache.get_device() == cur and out.get_device() == cur
+                and block_tables.get_device() == cur and seq_lens.get_device() == cur
+                and (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15 == 0
+                and blocks > 0 and max_blocks > 0 and (blocks + 1) * n_kv * PAGE < 1 << 31
+                and b * n_kv * (max_blocks // 2 + 2) < 1 << 31):
+            return b, n_q, n_kv, blocks, max_blocks
+    _check(q.dim() == 3 and q.shape[2] == 128 and q.dtype == _BF16, "q must be bf16 [batch, heads, 128]")
     b, n_q, _ = q.shape
-    _check(out.shape == q.shape and out.dtype == bf16, "out must be bf16 of q's shape")
+    _check(out.shape == q.shape and out.dtype == _BF16, "out must be bf16 of q's shape")
     for t in (q, out):
         _check(t.stride(2) == 1 and t.stride(1) == 128 and (t.stride(0) % 8 == 0 or b == 1) and t.data_ptr() % 16 == 0,
                "q and out must hold a row's heads next to each other, rows at multiples of 16 bytes")
     _check(b <= 1 or out.stride(0) >= n_q * 128, "out's rows overlap")
+    _check(b <= 1 or q.stride(0) > 0, "q's row stride must be positive")
     _check(k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (PAGE, 128) and k_cache.shape == v_cache.shape
-           and k_cache.dtype == bf16 and v_cache.dtype == bf16, f"caches must be bf16 [blocks, kv heads, {PAGE}, 128]")
-    _check(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+           and k_cache.dtype == _BF16 and v_cache.dtype == _BF16, f"caches must be bf16 [blocks, kv heads, {PAGE}, 128]")
+    _check(k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.data_ptr() % 16 == 0
+           and v_cache.data_ptr() % 16 == 0, "caches must be contiguous and 16-byte aligned")
     blocks, n_kv = k_cache.shape[:2]
     _check(blocks > 0 and (blocks + 1) * n_kv * PAGE < 1 << 31, "cache of no or too many blocks")
-    _check(block_tables.dtype == i32 and block_tables.dim() == 2 and block_tables.shape[0] == b
+    _check(block_tables.dtype == _I32 and block_tables.dim() == 2 and block_tables.shape[0] == b
            and block_tables.is_contiguous(), "block_tables must be contiguous int32 [batch, max_blocks]")
-    _check(seq_lens.dtype == i32 and tuple(seq_lens.shape) == (b,) and seq_lens.is_contiguous(),
+    _check(seq_lens.dtype == _I32 and tuple(seq_lens.shape) == (b,) and seq_lens.is_contiguous(),
            "seq_lens must be contiguous int32 [batch]")
     max_blocks = block_tables.shape[1]
     _check(0 < max_blocks and b * n_kv * (max_blocks // 2 + 2) < 1 << 31, "block_tables of no or too many pages")
@@ -83,16 +106,9 @@ def _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int
     return b, n_q, n_kv, blocks, max_blocks
 
 
-def _page_tmap(cache: torch.Tensor, box_rows: int) -> bytes:
-    """TMA map of a paged cache [blocks, Hkv, 64, 128] viewed as [rows, 128]:
-    64-column x ``box_rows`` boxes, 128B swizzle."""
-    rows = cache.shape[0] * cache.shape[1] * PAGE
-    return core().make_tmap_2d(cache.data_ptr(), 9, 128, rows, 256, 64, box_rows, 3)
-
-
-def span_grid(group: int) -> int:
+def span_ctas(group: int, sms: int) -> int:
     """CTAs of a decode launch: all that are resident at once."""
-    return _rt.sm_count() * (3 if group <= 8 else 2)
+    return sms * (3 if group <= 8 else 2)
 
 
 class SpanWorkspace:
@@ -112,11 +128,11 @@ class SpanWorkspace:
             device = device or torch.device("cuda", torch.cuda.current_device())
             empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
             zeros = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
-        self.ctas = 3 * _rt.sm_count()
-        pieces = max(2 * self.ctas * 8, 2 * span_grid(MAX_GROUP) * MAX_GROUP)  # (piece, head) pairs
+        self.sms = _rt.sm_count()
+        pieces = max(2 * span_ctas(g, self.sms) * p for g, p in ((8, 8), (16, 16)))  # (piece, head) pairs
         self.o = empty((pieces * 128,), torch.float32)
         self.ml = empty((pieces * 2,), torch.float32)
-        self.tickets = zeros((self.ctas,), torch.int32)
+        self.tickets = zeros((span_ctas(1, self.sms),), torch.int32)
         self.partials = partials
         self.prefix_o = empty((max(partials, 1) * 128,), torch.float32)
         self.prefix_ml = empty((max(partials, 1) * 2,), torch.float32)
@@ -129,13 +145,17 @@ def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, d
           scale: float, plan: "PrefixPlan | None") -> None:
     b, n_q, n_kv, blocks, max_blocks = dims
     g = n_q // n_kv
-    grid = min(span_grid(g), ws.ctas, b * n_kv * (max_blocks // 2 + 2))
-    _rt.launch(_SPAN, f"fb_span_attn_g{4 if g <= 4 else 8 if g <= 8 else 16}", (grid,), (192,), [
-        _page_tmap(k_cache, PAGE), _page_tmap(v_cache, PAGE), _page_tmap(k_cache, 16), _page_tmap(v_cache, 16),
-        q.data_ptr(), q.stride(0), block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(),
-        out.stride(0), b, n_kv, g, window, sinks, plan.row_info.data_ptr() if plan else 0, ws.prefix_o.data_ptr(),
-        ws.prefix_ml.data_ptr(), plan.parts if plan else 0, ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(),
-        float(scale * LOG2E)], smem=SPAN_SMEM)
+    k, v, rows = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE
+    if ws.tickets.get_device() != q.get_device():
+        raise ValueError("the workspace is on another device")
+    maps = core().make_tmaps_bf16([(k, 128, rows, 256, PAGE), (v, 128, rows, 256, PAGE),
+                                   (k, 128, rows, 256, 16), (v, 128, rows, 256, 16)])
+    _rt.launch(_SPAN, "fb_span_attn_g4" if g <= 4 else "fb_span_attn_g8" if g <= 8 else "fb_span_attn_g16",
+               (min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)),), (192,), [
+        maps, q.data_ptr(), q.stride(0), block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(),
+        out.data_ptr(), out.stride(0), b, n_kv, g, window, sinks, plan.row_info.data_ptr() if plan else 0,
+        ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), plan.parts if plan else 0, ws.o.data_ptr(), ws.ml.data_ptr(),
+        ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream())
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -147,7 +167,7 @@ def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Block-table entries of pages without a visible token are never read: their
     pages may have been freed. Rows of length 0 get zeros."""
-    dims = _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out)
+    dims = _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out)
     _check_group(dims[1], dims[2])
     _check_window(window, sinks)
     scale = _check_scale(scale)
@@ -211,9 +231,9 @@ class PrefixPlan:
             row += n
         self.items_n = len(items)
         self.partials = self.rows * n_q * self.parts  # (row, head, part) results that a SpanWorkspace has to hold
-        host = torch.tensor(items or [[0] * _ITEM], dtype=torch.int32), torch.tensor(info or [[0, 0]], dtype=torch.int32)
+        host = torch.tensor(items or [[0] * _ITEM], dtype=_I32), torch.tensor(info or [[0, 0]], dtype=_I32)
         if arena is not None:
-            self.items, self.row_info = (arena.empty(tuple(t.shape), torch.int32) for t in host)
+            self.items, self.row_info = (arena.empty(tuple(t.shape), _I32) for t in host)
             self.items.copy_(host[0])
             self.row_info.copy_(host[1])
         else:
@@ -229,24 +249,26 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     result and the arguments are those of ``decode_attention`` (``seq_lens``
     counts all tokens, ``block_tables`` begin with the shared pages). Rows of
     length 0 get zeros."""
-    dims = _check_decode(q, k_cache, v_cache, block_tables, seq_lens, out)
-    b, n_q, n_kv, blocks, max_blocks = dims
-    _check((plan.rows, plan.n_q, plan.n_kv, plan.max_blocks) == (b, n_q, n_kv, max_blocks),
-           f"plan for {plan.rows} rows, {plan.n_q} / {plan.n_kv} heads and {plan.max_blocks} pages, "
-           f"got {b}, {n_q} / {n_kv} and {max_blocks}")
-    _check(plan.partials <= ws.partials, f"workspace of {ws.partials} partial results, {plan.partials} needed")
-    _check_device(plan.items)
+    dims = b, n_q, n_kv, blocks, max_blocks = _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out)
+    if (plan.rows, plan.n_q, plan.n_kv, plan.max_blocks) != (b, n_q, n_kv, max_blocks):
+        raise ValueError(f"plan for {plan.rows} rows, {plan.n_q} / {plan.n_kv} heads and {plan.max_blocks} pages, "
+                         f"got {b}, {n_q} / {n_kv} and {max_blocks}")
+    if plan.partials > ws.partials:
+        raise ValueError(f"workspace of {ws.partials} partial results, {plan.partials} needed")
     scale = _check_scale(scale)
     if not b:
         return out
+    if plan.items.get_device() != q.get_device() or ws.tickets.get_device() != q.get_device():
+        raise ValueError("the plan or the workspace is on another device")
     if plan.items_n:
-        g = n_q // n_kv
-        q_map = core().make_tmap_2d(q.data_ptr(), 9, n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, 64,
-                                    prefix_rows(g), 3)
+        g, rows = n_q // n_kv, blocks * n_kv * PAGE
+        maps = core().make_tmaps_bf16([
+            (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g)),
+            (k_cache.data_ptr(), 128, rows, 256, PAGE), (v_cache.data_ptr(), 128, rows, 256, PAGE)])
         _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (128 * plan.tiles + 64,), [
-            q_map, _page_tmap(k_cache, PAGE), _page_tmap(v_cache, PAGE), plan.items.data_ptr(),
-            block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(),
-            g, n_q, n_kv, plan.parts, blocks, float(scale * LOG2E)], smem=TILE_SMEM[plan.tiles])
+            maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
+            ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, plan.parts, blocks, scale * LOG2E],
+            TILE_SMEM[plan.tiles], _rt.raw_stream())
     _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan)
     return out
 
@@ -260,26 +282,31 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     likewise with n_kv heads; out [T, n_q * 128]. The tile tables come from
     ``prefill_tiles(seqlens)``. Rows outside every prompt are neither used
     (they may hold anything) nor written."""
-    bf16, i32 = torch.bfloat16, torch.int32
     group = _check_group(n_q, n_kv)
     _check_window(window, sinks)
     scale = _check_scale(scale)
-    for t, heads, name in ((q, n_q, "q"), (k, n_kv, "k"), (v, n_kv, "v"), (out, n_q, "out")):
-        _check(t.dim() == 2 and t.dtype == bf16 and t.shape[1] >= heads * 128, f"{name} must be bf16 [T, >= {heads} * 128]")
-        _check(t.shape[0] == q.shape[0], f"{name} has {t.shape[0]} rows, q has {q.shape[0]}")
+    maps = []
     t = q.shape[0]
-    _check(out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0
-           and (t <= 1 or out.stride(0) >= n_q * 128), "out must be row-contiguous with 16-byte aligned rows")
+    for x, heads in ((q, n_q), (k, n_kv), (v, n_kv), (out, n_q)):
+        if not (x.dim() == 2 and x.dtype is _BF16 and x.shape[0] == t and x.shape[1] >= heads * 128):
+            raise ValueError(f"q, k, v and out must be bf16 [T, heads * 128] or wider, got {x.dtype} {tuple(x.shape)} for {heads} heads")
+        ld, inner = x.stride()
+        if t == 1:
+            ld = heads * 128
+        if inner != 1 or ld % 8 or ld < heads * 128 or x.data_ptr() % 16:
+            raise ValueError("q, k, v and out must be row-contiguous with 16-byte aligned rows that do not overlap")
+        maps.append((x.data_ptr(), heads * 128, t, ld * 2, TILE))
     for x in (cu_seqlens, tile_seq, tile_start):
-        _check(x.dtype == i32 and x.dim() == 1 and x.is_contiguous(), "cu_seqlens and the tile tables must be contiguous int32")
-    _check(tile_seq.numel() == tile_start.numel() and cu_seqlens.numel() >= 1, "tile tables of different lengths")
+        if not (x.dtype is _I32 and x.dim() == 1 and x.is_contiguous()):
+            raise ValueError("cu_seqlens and the tile tables must be contiguous int32")
+    n_tiles = tile_seq.shape[0]
+    if tile_start.shape[0] != n_tiles or cu_seqlens.shape[0] < 1:
+        raise ValueError("tile tables of different lengths, or no cu_seqlens")
     _check_device(q, k, v, out, cu_seqlens, tile_seq, tile_start)
-    n_tiles = tile_seq.numel()
     if not n_tiles or not t:
         return out
     qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
     _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (n_tiles, n_q // qt), (128 * qt + 64,), [
-        _rows_tmap(q[:, : n_q * 128]), _rows_tmap(k[:, : n_kv * 128]), _rows_tmap(v[:, : n_kv * 128]),
-        out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(), tile_start.data_ptr(), n_q, n_kv,
-        window, sinks, float(scale * LOG2E)], smem=TILE_SMEM[qt])
+        core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(),
+        tile_start.data_ptr(), n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
     return out
