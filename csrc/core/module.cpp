@@ -197,18 +197,19 @@ py::bytes rt_make_tmap_3d(uint64_t ptr, int dtype, uint64_t d0, uint64_t d1, uin
   return py::bytes(reinterpret_cast<const char*>(&m), sizeof(m));
 }
 
-// 2-D bf16 tensor maps with 64-column x box_rows boxes and the 128-byte swizzle,
-// one after another in one byte string (a kernel that needs several takes them
-// as one struct): (address, columns, rows, row stride in bytes, box rows) each.
-py::bytes rt_make_tmaps_bf16(const std::vector<std::array<uint64_t, 5>>& maps) {
+// bf16 tensor maps with 64-column x box_rows boxes and the 128-byte swizzle, one
+// after another in one byte string (a kernel that needs several takes them as
+// one struct): (address, columns, rows, row stride in bytes, box rows, planes,
+// plane stride in bytes) each; planes = 0 for two dimensions.
+py::bytes rt_make_tmaps_bf16(const std::vector<std::array<uint64_t, 7>>& maps) {
   std::vector<CUtensorMap> m(maps.size());
   for (size_t i = 0; i < maps.size(); ++i) {
     const auto& a = maps[i];
-    cuuint64_t dims[2] = {a[1], a[2]};
-    cuuint64_t strides[1] = {a[3]};
-    cuuint32_t box[2] = {64, static_cast<cuuint32_t>(a[4])};
-    cuuint32_t estr[2] = {1, 1};
-    check_drv(fb_driver()->cuTensorMapEncodeTiled(&m[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+    cuuint64_t dims[3] = {a[1], a[2], a[5]};
+    cuuint64_t strides[2] = {a[3], a[6]};
+    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a[4]), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    check_drv(fb_driver()->cuTensorMapEncodeTiled(&m[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a[5] ? 3 : 2,
                                                   reinterpret_cast<void*>(a[0]), dims, strides, box, estr,
                                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

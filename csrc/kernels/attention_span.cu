@@ -57,10 +57,9 @@ struct Smem {
   uint8_t q[QP_BYTES];
   uint8_t p[QP_BYTES];
   uint64_t kfull, vfull, kempty, vempty;
-  uint64_t s_full, s_empty, p_full, o_full, o_empty, q_ready;
-  float red[4][NH];      // per-warp max, then per-warp sum, of every head
-  float alpha[NH];       // this chunk's rescale factor per head
-  float mrun[2][NH];     // running max per head, by chunk parity
+  uint64_t s_full, s_empty, p_full, o_full, o_empty;
+  float red[4][NH];    // per-warp max, then per-warp sum, of every head
+  float mrun[2][NH];   // running max per head: one in use, one for the next move
   int scan[THREADS / 32];
   int total, first_row, first_off;
   uint32_t tmem;
@@ -81,19 +80,35 @@ __device__ __forceinline__ uint32_t qp_offset(int row, int k) {
   return (k >> 6) * (NH * 128) + row * 128 + (((kk >> 3) ^ (row & 7)) << 4) + (kk & 7) * 2;
 }
 
+// The softmax threads' barrier, and whether any of them brings true.
+__device__ __forceinline__ bool sync_softmax_or(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void sync_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// Caches viewed as [blocks * Hkv * 64, 128], K and V with boxes of a page x 64
+// dims, then K and V with boxes of 16 rows x 64 dims; q [B][Hq][128] with boxes
+// of one KV head's heads x 64 dims. 128B swizzle.
+struct SpanMaps {
+  CUtensorMap k, v, k16, v16, q;
+};
+
 struct Params {
-  const bf16* q;
   const int* block_tables;
   const int* seq_lens;
-  const int2* row_info;  // {tokens attended to by the prefix kernel, its parts} per row, or null
+  const int* row_prefix;  // tokens of each row that the prefix kernel has attended to, or null
   bf16* out;
-  const float *prefix_o, *prefix_ml;  // partial (row * Hq + head) * prefix_parts + part
+  const float *prefix_o, *prefix_ml;  // its results (row * Hq + head)
   float *ws_o, *ws_ml;                // [2 * gridDim][Hq / Hkv rounded up to the variant][128] and [..][2]
   int* tickets;                       // [gridDim], zero between launches
-  long long ld_q, ld_o;
-  int max_blocks, blocks, B, Hkv, G, prefix_parts, window, sinks;
+  long long ld_o;
+  int max_blocks, blocks, B, Hkv, G, window, sinks;
   float scale_log2;
 };
 
@@ -101,14 +116,20 @@ struct Params {
 // virtual pages 0 .. pages - 1: first those of the sinks, then from page `wp`.
 struct Span {
   int n, lo, sinks, sp, wp, pages, chunks;
+  bool prefix;  // the row has a partial result from the prefix kernel
   __device__ __forceinline__ int page(int v) const { return v < sp ? v : v - sp + wp; }
 };
 
-__device__ __forceinline__ Span row_span(const Params& a, int b) {
+// (length, prefix tokens) of a row; a row behind the last one is empty.
+__device__ __forceinline__ int2 row_length(const Params& a, int b) {
+  return b < a.B ? make_int2(a.seq_lens[b], a.row_prefix ? a.row_prefix[b] : 0) : make_int2(0, 0);
+}
+
+__device__ __forceinline__ Span row_span(const Params& a, int2 length) {
   Span s;
-  s.n = min(max(a.seq_lens[b], 0), a.max_blocks * PAGE);
-  const int start = a.row_info ? min(a.row_info[b].x, s.n) : 0;
-  s.lo = a.window > 0 ? max(s.n - a.window, 0) : start;
+  s.n = min(max(length.x, 0), a.max_blocks * PAGE);
+  s.prefix = length.y > 0;
+  s.lo = a.window > 0 ? max(s.n - a.window, 0) : min(length.y, s.n);
   s.sinks = a.window > 0 ? min(a.sinks, s.lo) : 0;
   s.sp = (s.sinks + PAGE - 1) / PAGE;
   s.wp = max(s.sp, s.lo / PAGE);
@@ -122,11 +143,11 @@ __device__ __forceinline__ Span row_span(const Params& a, int b) {
 struct Walk {
   int b, kvh, c0, c1, at, end;
   Span s;
-  bool fresh;
-  __device__ __forceinline__ Walk(const Params& a, const Smem& sm, int begin, int e)
-      : b(sm.first_row), at(begin), end(e), fresh(true) {
+  int2 ahead;  // the next row's length, read a row ahead: off the critical path
+  __device__ __forceinline__ Walk(const Params& a, const Smem& sm, int begin, int e) : b(sm.first_row), at(begin), end(e) {
     if (begin >= end) return;
-    s = row_span(a, b);
+    s = row_span(a, row_length(a, b));
+    ahead = row_length(a, b + 1);
     kvh = sm.first_off / s.chunks;
     c0 = sm.first_off % s.chunks;
     c1 = min(s.chunks, c0 + end - at);
@@ -138,15 +159,62 @@ struct Walk {
     c0 = 0;
     if (++kvh == a.Hkv) {
       kvh = 0;
-      s = row_span(a, ++b);
+      s = row_span(a, ahead);
+      ahead = row_length(a, ++b + 1);
     }
     c1 = min(s.chunks, end - at);
   }
 };
 
+__device__ __forceinline__ int add_acq_rel(int* p, int v) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
+// Joins n partial results (max, sum) = *ml(k, h), output *part(k, h) into (m, l,
+// o) of two heads h = 0, 1. The loads of JOIN parts of both are on their way at a
+// time: one by one, their latency is what the join would take.
+constexpr int JOIN = 4;
+template <class Ml, class Part>
+__device__ __forceinline__ void join_parts(float (&m)[2], float (&l)[2], float (&o)[2], int n, Ml ml, Part part) {
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += JOIN) {
+    float2 s[JOIN][2];
+    float v[JOIN][2];
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[k][h] = __ldcg(ml(min(k0 + k, n - 1), h));  // without a branch, so that none waits for another
+        v[k][h] = __ldcg(part(min(k0 + k, n - 1), h));
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = m[h];
+#pragma unroll
+      for (int k = 1; k < JOIN; ++k)
+        if (k0 + k >= n) s[k][h] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < JOIN; ++k) mx = fmaxf(mx, s[k][h].x);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float w = exp2f(m[h] - ref);
+      l[h] *= w;
+      o[h] *= w;
+#pragma unroll
+      for (int k = 0; k < JOIN; ++k) {
+        const float e = exp2f(s[k][h].x - ref);
+        l[h] = fmaf(s[k][h].y, e, l[h]);
+        o[h] = e > 0.f ? fmaf(v[k][h], e, o[h]) : o[h];
+      }
+      m[h] = mx;
+    }
+  }
+}
+
 template <int GP>
-__device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensorMap* tmV, const CUtensorMap* tmK16,
-                                          const CUtensorMap* tmV16, const Params& a) {
+__device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a) {
+  const CUtensorMap *tmK = &maps.k, *tmV = &maps.v, *tmK16 = &maps.k16, *tmV16 = &maps.v16;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -161,7 +229,6 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
     mbar_init(&sm.s_empty, 4);
     mbar_init(&sm.p_full, 4);
     mbar_init(&sm.o_empty, 4);
-    mbar_init(&sm.q_ready, 4);
     sm.abort = sm.give_up = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -169,12 +236,14 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
     tma_prefetch_desc(tmV);
     tma_prefetch_desc(tmK16);
     tma_prefetch_desc(tmV16);
+    tma_prefetch_desc(&maps.q);
   }
   if (warp == 1) {
     tmem_alloc(&sm.tmem, 32);
     tmem_relinquish();
   }
-  // Rows of heads >= G stay zero for the whole kernel.
+  // Rows of heads >= G are never written: zeros, if only so that what the
+  // products make of them is finite (each head's column depends on its own row).
   for (int i = threadIdx.x; i < QP_BYTES / 16; i += THREADS) {
     reinterpret_cast<uint4*>(sm.p)[i] = make_uint4(0, 0, 0, 0);
     reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
@@ -191,7 +260,7 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
   const int row0 = min(static_cast<int>(threadIdx.x) * R, a.B), row1 = min(row0 + R, a.B);
   int mine = 0;
   for (int b = row0; b < row1; ++b) {
-    mine += row_span(a, b).chunks * a.Hkv;
+    mine += row_span(a, row_length(a, b)).chunks * a.Hkv;
     if (blockIdx.x == 0 && (a.seq_lens[b] < 0 || a.seq_lens[b] > a.max_blocks * PAGE)) set_status(FB_KERR_BAD_ARG);
   }
   int incl = mine;
@@ -212,7 +281,7 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
   if (begin < end && begin >= before && begin < before + mine) {
     int off = begin - before, b = row0;
     for (;; ++b) {
-      const int len = row_span(a, b).chunks * a.Hkv;
+      const int len = row_span(a, row_length(a, b)).chunks * a.Hkv;
       if (off < len) break;
       off -= len;
     }
@@ -261,7 +330,12 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
               sm.abort = 1;
               continue;  // no copies for this chunk; the loop ends below
             }
-            mbar_arrive_expect_tx(full, bytes);
+            // An item's q rows come with its first K: the last item's Q K^T is done by then.
+            const bool first = kv == 0 && c == w.c0;
+            mbar_arrive_expect_tx(full, bytes + (first ? a.G * D * 2 : 0));
+            if (first)
+              for (int hf = 0; hf < 2; ++hf)
+                tma_load_3d(sm.q + hf * (NH * 128), &maps.q, full, hf * 64, w.kvh * a.G, w.b);
             uint8_t* buf = kv ? sm.v : sm.k;
 #pragma unroll
             for (int pg = 0; pg < 2; ++pg) {
@@ -290,14 +364,9 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
       const uint32_t kb = smem_u32(sm.k), vb = smem_u32(sm.v), qb = smem_u32(sm.q), pb = smem_u32(sm.p);
-      uint32_t cc = 0, items = 0;  // chunks and pieces so far
+      uint32_t cc = 0;  // chunks so far
       bool ok = true;
       for (Walk w(a, sm, begin, end); ok && w.more() && !*(volatile int*)&sm.abort; w.next(a)) {
-        if (!mbar_wait(&sm.q_ready, items & 1, FB_KERR_TIMEOUT_FULL)) {
-          ok = false;
-          break;
-        }
-        ++items;
         for (int c = w.c0; c < w.c1; ++c, ++cc) {
           if (!mbar_wait(&sm.kfull, cc & 1, FB_KERR_TIMEOUT_FULL) ||
               !mbar_wait(&sm.s_empty, (cc & 1) ^ 1, FB_KERR_TIMEOUT_TMEM)) {
@@ -339,24 +408,21 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const int G = a.G, Hq = a.Hkv * G;
     uint32_t cc = 0;
+    int cur = 0;  // which of mrun is in use (the same in all threads)
     volatile int* give_up = &sm.give_up;
     for (Walk w(a, sm, begin, end); w.more(); w.next(a)) {
-      for (int e = r; e < G * 16; e += 128) {  // the heads' q rows, 16 B at a time
-        const int row = e >> 4, col = (e & 15) * 8;
-        *reinterpret_cast<uint4*>(sm.q + qp_offset(row, col)) =
-            *reinterpret_cast<const uint4*>(a.q + w.b * a.ld_q + (w.kvh * G + row) * D + col);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_ready);
-
       float l_thr[GP], o[GP];
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        // chunk k reads mrun[k & 1]; thread 0 writes the next one's after the first barrier of chunk k
-        if (r == 0) sm.mrun[cc & 1][g] = -INFINITY;
-        l_thr[g] = 0.f;
+        float2 ml = make_float2(-INFINITY, 0.f);
         o[g] = 0.f;
+        if (w.s.prefix && w.c0 == 0 && g < G) {  // the item's first piece goes on from the prefix's result
+          const size_t at = static_cast<size_t>(w.b) * Hq + w.kvh * G + g;
+          ml = *(reinterpret_cast<const float2*>(a.prefix_ml) + at);
+          o[g] = a.prefix_o[at * D + r];
+        }
+        if (r == 0) sm.mrun[cur][g] = ml.x;
+        l_thr[g] = r == 0 ? ml.y : 0.f;
       }
       for (int c = w.c0; c < w.c1; ++c, ++cc) {
         if (!mbar_wait(&sm.s_full, cc & 1, FB_KERR_TIMEOUT_TMEM)) *give_up = 1;
@@ -381,32 +447,46 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
             for (int i = 0; i < 8; ++i)
               reinterpret_cast<uint4*>(vrow + h * HALF_STRIDE)[i] = make_uint4(0, 0, 0, 0);
         }
+        // The maxima move only if a score is above one by more than 8 (log2
+        // units: p stays below 256, exact in the fp32 sums), and in a piece's
+        // first chunk: the reduction over the tokens is for those chunks alone.
+        bool move = c == w.c0;
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           const float s = valid ? __uint_as_float(sr[g]) * a.scale_log2 : -INFINITY;
           sr[g] = __float_as_uint(s);
-          const float cmax = warp_max(s);
-          if (lane == 0) sm.red[quarter][g] = cmax;
+          move |= g < G && c > w.c0 && s > sm.mrun[cur][g] + 8.f;
         }
-        sync_softmax();
+        move = sync_softmax_or(move);
         if (*give_up) break;  // the same in every softmax thread: written only outside this pair of barriers
+        if (move) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float cmax = warp_max(__uint_as_float(sr[g]));
+            if (lane == 0) sm.red[quarter][g] = cmax;
+          }
+          sync_softmax();
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float mx = fmaxf(fmaxf(sm.red[0][g], sm.red[1][g]), fmaxf(sm.red[2][g], sm.red[3][g]));
+            const float m_old = sm.mrun[cur][g], m_new = fmaxf(m_old, mx);
+            const float alpha = exp2f(m_old - (m_new == -INFINITY ? 0.f : m_new));
+            if (r == 0) sm.mrun[cur ^ 1][g] = m_new;
+            l_thr[g] *= alpha;
+            o[g] *= alpha;
+          }
+          cur ^= 1;
+          sync_softmax();  // mrun is read below
+        }
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float mx = fmaxf(fmaxf(sm.red[0][g], sm.red[1][g]), fmaxf(sm.red[2][g], sm.red[3][g]));
-          const float m_old = sm.mrun[cc & 1][g];
-          const float m_new = fmaxf(m_old, mx);
-          const float m_use = m_new == -INFINITY ? 0.f : m_new;
-          const float alpha = exp2f(m_old - m_use);
-          if (r == 0) {
-            sm.alpha[g] = alpha;
-            sm.mrun[(cc + 1) & 1][g] = m_new;
-          }
-          const float p = exp2f(__uint_as_float(sr[g]) - m_use);
-          l_thr[g] = l_thr[g] * alpha + p;
+          const float m = sm.mrun[cur][g];
+          const float p = exp2f(__uint_as_float(sr[g]) - (m == -INFINITY ? 0.f : m));
+          l_thr[g] += p;
           if (g < G) *reinterpret_cast<bf16*>(sm.p + qp_offset(g, r)) = f2bf(p);
         }
         fence_proxy_async();
-        sync_softmax();  // red and alpha are rewritten next chunk
+        sync_softmax();
         if (lane == 0) mbar_arrive(&sm.p_full);
         if (!mbar_wait(&sm.o_full, cc & 1, FB_KERR_TIMEOUT_TMEM)) *give_up = 1;
         tc_fence_after();
@@ -417,7 +497,7 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.o_empty);
 #pragma unroll
-        for (int g = 0; g < GP; ++g) o[g] = o[g] * sm.alpha[g] + __uint_as_float(orr[g]);
+        for (int g = 0; g < GP; ++g) o[g] += __uint_as_float(orr[g]);
       }
       // Sum of a head over the 128 token lanes.
 #pragma unroll
@@ -427,13 +507,10 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
       }
       sync_softmax();
       if (*give_up) break;  // again the same in every thread; the workspace's tickets are then left as they are
-      float m[GP], l[GP];
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        l[g] = (sm.red[0][g] + sm.red[1][g]) + (sm.red[2][g] + sm.red[3][g]);
-        m[g] = sm.mrun[cc & 1][g];
-      }
-      // This piece's item starts at flat position `at0` and lies in the shares of CTAs [f, e].
+      // Every thread of the piece's heads: their max and sum (the same in all), its dim of their outputs.
+      auto own_m = [&](int g) { return sm.mrun[cur][g]; };
+      auto own_l = [&](int g) { return (sm.red[0][g] + sm.red[1][g]) + (sm.red[2][g] + sm.red[3][g]); };
+      // This piece's item starts at flat position `at0` and lies in the shares of CTAs f, f + 1, ..
       const int at0 = w.at - w.c0, f = at0 / share, pieces = (at0 + w.s.chunks - 1) / share - f + 1;
       bool finish = true;
       if (pieces > 1) {
@@ -441,57 +518,41 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           __stcg(a.ws_o + (slot * GP + g) * D + r, o[g]);
-          if (r == 0) __stcg(reinterpret_cast<float2*>(a.ws_ml) + slot * GP + g, make_float2(m[g], l[g]));
+          if (r == 0) __stcg(reinterpret_cast<float2*>(a.ws_ml) + slot * GP + g, make_float2(own_m(g), own_l(g)));
         }
-        __threadfence();
         sync_softmax();
         if (r == 0) {
-          __threadfence();
-          const int done = atomicAdd(a.tickets + f, 1) + 1;
+          // releases the warps' writes (ordered before it by the barrier), acquires the other pieces'
+          const int done = add_acq_rel(a.tickets + f, 1) + 1;
           sm.last = done == pieces;
           if (done == pieces) a.tickets[f] = 0;
-          __threadfence();
         }
         sync_softmax();
         finish = sm.last;
-        if (finish) {
-#pragma unroll
-          for (int g = 0; g < GP; ++g) {
-            m[g] = -INFINITY;
-            l[g] = o[g] = 0.f;
-          }
-          for (int k = 0; k < pieces; ++k) {
-            const size_t from = 2 * static_cast<size_t>(f + k) + (k == 0 && at0 % share ? 1 : 0);
-#pragma unroll
-            for (int g = 0; g < GP; ++g) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + from * GP + g);
-              const float op = __ldcg(a.ws_o + (from * GP + g) * D + r);
-              const float mx = fmaxf(m[g], ml.x), ref = mx == -INFINITY ? 0.f : mx;
-              const float w0 = exp2f(m[g] - ref), w1 = exp2f(ml.x - ref);
-              l[g] = l[g] * w0 + ml.y * w1;
-              o[g] = o[g] * w0 + op * w1;
-              m[g] = mx;
-            }
-          }
-        }
       }
       if (finish) {
-        const int np = a.row_info ? a.row_info[w.b].y : 0;
+        const int odd = at0 % share ? 1 : 0;  // the first piece is its CTA's last
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
+        for (int g = 0; g < GP; g += 2) {
           if (g >= G) break;
-          const int hq = w.kvh * G + g;
-          const size_t at = (static_cast<size_t>(w.b) * Hq + hq) * a.prefix_parts;
-          for (int k = 0; k < np; ++k) {
-            const float2 ml = *(reinterpret_cast<const float2*>(a.prefix_ml) + at + k);
-            const float op = a.prefix_o[(at + k) * D + r];
-            const float mx = fmaxf(m[g], ml.x), ref = mx == -INFINITY ? 0.f : mx;
-            const float w0 = exp2f(m[g] - ref), w1 = exp2f(ml.x - ref);
-            l[g] = l[g] * w0 + ml.y * w1;
-            o[g] = o[g] * w0 + op * w1;
-            m[g] = mx;
+          float m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.f, 0.f}, o2[2] = {0.f, 0.f};
+          if (pieces == 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              m2[h] = own_m(g + h);
+              l2[h] = own_l(g + h);
+              o2[h] = o[g + h];
+            }
+          } else {
+            auto slot = [&](int k) { return (2 * static_cast<size_t>(f + k) + (k == 0 ? odd : 0)) * GP + g; };
+            join_parts(
+                m2, l2, o2, pieces,
+                [&](int k, int h) { return reinterpret_cast<const float2*>(a.ws_ml) + slot(k) + h; },
+                [&](int k, int h) { return a.ws_o + (slot(k) + h) * D + r; });
           }
-          a.out[w.b * a.ld_o + hq * D + r] = f2bf(l[g] > 0.f ? o[g] / l[g] : 0.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (g + h < G) a.out[w.b * a.ld_o + (w.kvh * G + g + h) * D + r] = f2bf(l2[h] > 0.f ? o2[h] / l2[h] : 0.f);
         }
       }
       sync_softmax();  // red, mrun and last are rewritten by the next piece
@@ -507,22 +568,15 @@ __device__ __forceinline__ void span_body(const CUtensorMap* tmK, const CUtensor
 
 }  // namespace
 
-// Caches viewed as [blocks * Hkv * 64, 128], K and V with boxes of a page x 64
-// dims, then K and V with boxes of 16 rows x 64 dims, 128B swizzle.
-struct SpanMaps {
-  CUtensorMap k, v, k16, v16;
-};
-
 #define FB_SPAN_INSTANCE(GP, CTAS)                                                                                \
   extern "C" __global__ void __launch_bounds__(THREADS, CTAS) fb_span_attn_g##GP(                                 \
-      const __grid_constant__ SpanMaps maps, const bf16* q, long long ld_q, const int* block_tables,              \
-      int max_blocks, int blocks, const int* seq_lens, bf16* out, long long ld_o, int B, int Hkv, int G,          \
-      int window, int sinks, const int2* row_info, const float* prefix_o, const float* prefix_ml,                 \
-      int prefix_parts, float* ws_o, float* ws_ml, int* tickets, float scale_log2) {                              \
-    const Params a{q,     block_tables, seq_lens, row_info, out, prefix_o, prefix_ml,    ws_o,   ws_ml, tickets,  \
-                   ld_q,  ld_o,         max_blocks, blocks, B,   Hkv,      G,            prefix_parts, window,    \
-                   sinks, scale_log2};                                                                            \
-    span_body<GP>(&maps.k, &maps.v, &maps.k16, &maps.v16, a);                                                     \
+      const __grid_constant__ SpanMaps maps, const int* block_tables, int max_blocks, int blocks,                 \
+      const int* seq_lens, bf16* out, long long ld_o, int B, int Hkv, int G, int window, int sinks,               \
+      const int* row_prefix, const float* prefix_o, const float* prefix_ml, float* ws_o, float* ws_ml,            \
+      int* tickets, float scale_log2) {                                                                           \
+    const Params a{block_tables, seq_lens, row_prefix, out,    prefix_o, prefix_ml, ws_o,   ws_ml, tickets,       \
+                   ld_o,         max_blocks, blocks,   B,      Hkv,      G,         window, sinks, scale_log2};   \
+    span_body<GP>(maps, a);                                                                                       \
   }
 
 FB_SPAN_INSTANCE(4, 3)

@@ -6,9 +6,12 @@
 //                             j < sinks); writes bf16 rows
 //   fb_prefix_attn_q{1,2}     a decode batch against pages that a group of its
 //                             sequences shares: the group's queries x G heads
-//                             of one KV head are the rows of the tile; writes
-//                             unnormalised fp32 partials and (max, sum) for
-//                             the join in attention_span.cu
+//                             of one KV head are the rows of the tile. The
+//                             pages are split over the CTAs of a cluster, which
+//                             join their results through each other's shared
+//                             memory; writes one unnormalised fp32 result and
+//                             (max, sum) per row and head, from which
+//                             attention_span.cu goes on
 //
 // Per key tile and 128-row query tile:
 //   S = Q K^T          tcgen05.mma M=128 N=128 K=128, both from shared memory
@@ -51,6 +54,7 @@ constexpr int HALF = 128 * 128;      // one 64-dim half of a 128-row tile: 128 r
 constexpr int TILE = 2 * HALF;       // 128 rows x 128 dims bf16
 constexpr float RESCALE_LOG2 = 8.f;  // lazy-rescale threshold
 constexpr int EVERY_KEY = 0x3fffffff;
+constexpr int MAX_CLUSTER = 8;
 
 template <int QT>
 struct Smem {
@@ -61,9 +65,45 @@ struct Smem {
   uint64_t s_full[QT], p_full[QT], o_full[QT];
   uint32_t tmem;
   int abort;
+  // (max, sum) of each row for the cluster's join: in q's memory, when the products are done
+  __device__ __forceinline__ float2* ml(int t) { return reinterpret_cast<float2*>(q[0]) + t * BQ; }
 };
 static_assert(sizeof(Smem<2>) + 1024 <= 226 * 1024, "host requests 226 KB of dynamic shared memory (2 tiles)");
 static_assert(sizeof(Smem<1>) + 1024 <= 98 * 1024, "host requests 98 KB of dynamic shared memory (1 tile)");
+
+// ---- thread-block clusters ----
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared variable in the CTA of rank `rank`.
+__device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 load_remote4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_remote2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
 
 // What the body needs of a CTA's work: n key tiles, tile i starting at key
 // position key0(i); loads; and each row's visible keys
@@ -100,7 +140,10 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
   pdl_trigger();  // not before: a dependent's CTA must not take TMEM that this one has yet to allocate
   const uint32_t tmem = sm.tmem;  // S_t at columns 128 t, O_t at 128 (QT + t)
 
-  if (warp == 4 * QT) {
+  if (n == 0) {
+    // nothing for this CTA of a cluster (w.finish below still counts on it)
+    if (warp < 4 * QT) sm.ml(warp >> 2)[threadIdx.x & 127] = make_float2(-INFINITY, 0.f);
+  } else if (warp == 4 * QT) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
       w.load_q(sm, &sm.q_full);
@@ -282,13 +325,16 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[t]);
     }
-    if (ok && mbar_wait(&sm.o_full[t], 0, FB_KERR_TIMEOUT_TMEM)) {
+    for (int i = 0; ok && i < QT; ++i)  // of every tile: a store may reuse the ring
+      if (i == t || Work::REUSES_RING) ok = mbar_wait(&sm.o_full[i], 0, FB_KERR_TIMEOUT_TMEM);
+    if (ok) {
       tc_fence_after();
-      w.store(t, r, t_o, m_run, l_run);
+      w.store(sm, t, r, t_o, m_run, l_run);
     } else {
       sm.abort = 1;
     }
   }
+  w.finish(sm);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -328,7 +374,9 @@ struct WindowWork {
     hi = s0 + qpos < s1 ? qpos : -1;
     lo = qpos - window + 1;
   }
-  __device__ __forceinline__ void store(int t, int r, uint32_t t_o, float, float l) const {
+  static constexpr bool REUSES_RING = false;
+  __device__ __forceinline__ void finish(Smem<QT>&) const {}
+  __device__ __forceinline__ void store(Smem<QT>&, int t, int r, uint32_t t_o, float, float l) const {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const bool live = s0 + qp0 + r < s1;
     bf16* row = out + static_cast<size_t>(s0 + qp0 + r) * ld_o + (head0 + t) * D;
@@ -385,13 +433,13 @@ __device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUt
 }
 
 // ---- shared prefix of a decode batch ---------------------------------------------------
-// items[blockIdx.x] = {first row, rows, first page, pages, part, 0, 0, 0}: the rows
-// (sequences) of one group against a range of the pages that its first row's
-// block table begins with. Row r of query tile t is head r / nb of the group's
+// items[blockIdx.x] = {first row, rows, first page, pages}: the rows (sequences)
+// of one group against a range of the pages that its first row's block table
+// begins with; the CTAs of a cluster have the same rows. Row r of query tile t is head r / nb of the group's
 // KV head for sequence first + t * nb + r % nb, nb = 128 / G rounded down to a
 // multiple of 8 (whole swizzle atoms), so one TMA box of nb rows fetches one head.
 struct PrefixItem {
-  int row0, rows, page0, pages, part, pad[3];
+  int row0, rows, page0, pages;
 };
 
 template <int QT>
@@ -400,7 +448,7 @@ struct PrefixWork {
   const int *pages, *seq_lens;
   float *o_part, *ml_part;
   PrefixItem it;
-  int kvh, G, nb, Hq, Hkv, parts, blocks;
+  int kvh, G, nb, Hq, Hkv, blocks;
   int n, sinks;
 
   __device__ __forceinline__ int key0(int i) const { return it.page0 * PAGE + i * BK; }
@@ -443,23 +491,68 @@ struct PrefixWork {
     hi = r < G * nb && b < it.rows ? min(seq_lens[it.row0 + b], end) - 1 : EVERY_KEY;
     lo = 0;
   }
-  __device__ __forceinline__ void store(int t, int r, uint32_t t_o, float m, float l) const {
+  // Index of a tile row's result; -1 if no head and sequence uses it.
+  __device__ __forceinline__ long long result_of(int t, int r) const {
     const int b = row_of(t, r);
-    const bool live = r < G * nb && b < it.rows;
-    const size_t at = (static_cast<size_t>(it.row0 + b) * Hq + kvh * G + r / nb) * parts + it.part;
-    if (live) *reinterpret_cast<float2*>(ml_part + 2 * at) = make_float2(m, l);
-    float* row = o_part + at * D;
+    return r < G * nb && b < it.rows ? (it.row0 + b) * static_cast<long long>(Hq) + kvh * G + r / nb : -1;
+  }
+  static constexpr bool REUSES_RING = true;
+  // O rows of the tiles in the ring's memory, 16-byte chunks swizzled by the row.
+  __device__ __forceinline__ static uint32_t o_at(Smem<QT>& sm, int t, int r, int chunk) {
+    return smem_u32(sm.kv[0]) + (t * BQ + r) * (D * 4) + ((chunk ^ (r & 31)) << 4);
+  }
+  __device__ __forceinline__ void store(Smem<QT>& sm, int t, int r, uint32_t t_o, float m, float l) const {
+    sm.ml(t)[r] = make_float2(m, l);
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
       tmem_ld32(t_o + c, o);
       tmem_ld_wait();
-      if (live) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<uint4*>(row + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-      }
+      for (int e = 0; e < 32; e += 4)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(o_at(sm, t, r, (c + e) / 4)), "r"(o[e]),
+                     "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3])
+                     : "memory");
     }
+  }
+  // The cluster's CTAs have the same rows: a warp joins one row at a time, of
+  // the rows that fall to its CTA.
+  __device__ __forceinline__ void finish(Smem<QT>& sm) const {
+    cluster_sync();
+    const int size = cluster_size(), warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    for (int i = cluster_rank() * warps + (threadIdx.x >> 5); i < QT * BQ; i += size * warps) {
+      const int t = i / BQ, r = i % BQ;
+      const long long at = result_of(t, r);
+      if (at < 0) continue;
+      float2 ml[MAX_CLUSTER];
+      float4 o[MAX_CLUSTER];
+      float m = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < MAX_CLUSTER; ++c) {
+        ml[c] = make_float2(-INFINITY, 0.f);
+        if (c < size) {
+          ml[c] = load_remote2(map_to(smem_u32(sm.ml(t) + r), c));
+          o[c] = load_remote4(map_to(o_at(sm, t, r, lane), c));
+        }
+        m = fmaxf(m, ml[c].x);
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < MAX_CLUSTER; ++c) {
+        const float e = exp2f(ml[c].x - ref);
+        if (!(e > 0.f)) continue;  // (an empty part's O is no number)
+        l = fmaf(ml[c].y, e, l);
+        sum.x = fmaf(o[c].x, e, sum.x);
+        sum.y = fmaf(o[c].y, e, sum.y);
+        sum.z = fmaf(o[c].z, e, sum.z);
+        sum.w = fmaf(o[c].w, e, sum.w);
+      }
+      reinterpret_cast<float4*>(o_part + at * D)[lane] = sum;
+      if (lane == 0) *reinterpret_cast<float2*>(ml_part + 2 * at) = make_float2(m, l);
+    }
+    cluster_sync();  // the others may still be reading this CTA's shared memory
   }
 };
 
@@ -467,12 +560,11 @@ template <int QT>
 __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const CUtensorMap* tmK,
                                                  const CUtensorMap* tmV, const PrefixItem* items,
                                                  const int* block_tables, int max_blocks, const int* seq_lens,
-                                                 float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts,
-                                                 int blocks, float scale_log2) {
+                                                 float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks,
+                                                 float scale_log2) {
   pdl_wait();
   PrefixWork<QT> w;
   w.it = items[blockIdx.x];
-  if (w.it.pages <= 0) return;
   w.tmQ = tmQ;
   w.tmK = tmK;
   w.tmV = tmV;
@@ -485,7 +577,6 @@ __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const C
   w.nb = (128 / G) & ~7;
   w.Hq = Hq;
   w.Hkv = Hkv;
-  w.parts = parts;
   w.blocks = blocks;
   w.n = (w.it.pages + 1) / 2;
   w.sinks = 0;
@@ -518,15 +609,14 @@ FB_WINDOW_PREFILL(1, 2)
 FB_WINDOW_PREFILL(2, 1)
 
 // q [B, Hq * 128] with boxes of nb rows; caches viewed as [blocks * Hkv * 64,
-// 128] with boxes of one page. Grid: (items, Hkv). Partial `part` of (row, head)
-// at index (row * Hq + head) * parts + part.
+// 128] with boxes of one page. Grid: (items, Hkv), clusters of the items that
+// share their rows. The result of (row, head) is at index row * Hq + head.
 #define FB_PREFIX_ATTN(QT, CTAS)                                                                                  \
   extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_prefix_attn_q##QT(                         \
       const __grid_constant__ TileMaps maps, const PrefixItem* items, const int* block_tables, int max_blocks,    \
-      const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts, int blocks,          \
-      float scale_log2) {                                                                                         \
+      const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks, float scale_log2) {      \
     prefix_attention<QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \
-                         G, Hq, Hkv, parts, blocks, scale_log2);                                                  \
+                         G, Hq, Hkv, blocks, scale_log2);                                                         \
   }
 FB_PREFIX_ATTN(1, 2)
 FB_PREFIX_ATTN(2, 1)

@@ -26,7 +26,7 @@ MAX_GROUP = 16
 SPAN_SMEM = 74 * 1024
 TILE_SMEM = {1: 98 * 1024, 2: 226 * 1024}
 TILE = 128  # queries (and keys) of a tile
-_ITEM = 8  # int32 words of a prefix work item
+MAX_CLUSTER = 8  # CTAs that share a prefix's pages between them
 _BF16, _I32 = torch.bfloat16, torch.int32
 
 
@@ -113,8 +113,8 @@ def span_ctas(group: int, sms: int) -> int:
 
 class SpanWorkspace:
     """Partial results of the decode calls: two pieces per CTA (the same for
-    every batch and length), and ``partials`` (row, head, part) results of
-    shared prefixes (``PrefixPlan.partials``; 0 if there are none). With
+    every batch and length), and the results of shared prefixes for
+    ``partials`` (row, head) pairs (``PrefixPlan.partials``). With
     ``arena`` the buffers come from it (a runner whose graphs are saved).
 
     Calls that may run at the same time need a workspace each; calls in stream
@@ -146,16 +146,18 @@ def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, d
     b, n_q, n_kv, blocks, max_blocks = dims
     g = n_q // n_kv
     k, v, rows = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE
+    ld = q.stride(0) if b > 1 else n_q * 128
     if ws.tickets.get_device() != q.get_device():
         raise ValueError("the workspace is on another device")
-    maps = core().make_tmaps_bf16([(k, 128, rows, 256, PAGE), (v, 128, rows, 256, PAGE),
-                                   (k, 128, rows, 256, 16), (v, 128, rows, 256, 16)])
+    # q last: its heads are a dimension of their own (one box: a KV head's heads of one row)
+    maps = core().make_tmaps_bf16([(k, 128, rows, 256, PAGE, 0, 0), (v, 128, rows, 256, PAGE, 0, 0),
+                                   (k, 128, rows, 256, 16, 0, 0), (v, 128, rows, 256, 16, 0, 0),
+                                   (q.data_ptr(), 128, n_q, 256, g, b, ld * 2)])
     _rt.launch(_SPAN, "fb_span_attn_g4" if g <= 4 else "fb_span_attn_g8" if g <= 8 else "fb_span_attn_g16",
                (min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)),), (192,), [
-        maps, q.data_ptr(), q.stride(0), block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(),
-        out.data_ptr(), out.stride(0), b, n_kv, g, window, sinks, plan.row_info.data_ptr() if plan else 0,
-        ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), plan.parts if plan else 0, ws.o.data_ptr(), ws.ml.data_ptr(),
-        ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream())
+        maps, block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv,
+        g, window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(),
+        ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream())
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -182,12 +184,12 @@ def prefix_rows(group: int) -> int:
 
 
 def _prefix_splits(tiles: int, pages: int, slots: int) -> int:
-    """Parts that the ``pages`` of a prefix are cut into, ``tiles`` CTAs each:
-    the cut with the shortest schedule of ``slots`` CTAs at a time, where a
-    part costs its key tiles and about three more for its start and its end."""
+    """CTAs of a cluster that share the ``pages`` of a prefix, for ``tiles``
+    clusters: those with the shortest schedule of ``slots`` CTAs at a time,
+    where a CTA costs its key tiles and about three more for its start and end."""
     keys = math.ceil(pages / 2)
-    best = min((math.ceil(tiles * s / slots) * (math.ceil(keys / s) + 3), s) for s in range(1, min(keys, 64) + 1))
-    return best[1]
+    return min((math.ceil(tiles * s / slots) * (math.ceil(keys / s) + 3), s)
+               for s in (1, 2, 4, MAX_CLUSTER) if s <= max(keys, 1))[1]
 
 
 class PrefixPlan:
@@ -214,31 +216,27 @@ class PrefixPlan:
         self.tiles = 2 if any(n > nb for n, _ in shared) else 1
         step = nb * self.tiles
         slots = max(1, _rt.sm_count() * (1 if self.tiles == 2 else 2) // n_kv)
-        ctas = sum(math.ceil(n / step) for n, _ in shared)
-        items, info, row, self.parts = [], [], 0, 0
+        clusters = sum(math.ceil(n / step) for n, _ in shared)
+        self.splits = _prefix_splits(clusters, max((p for _, p in shared), default=0), slots)
+        items, info, row = [], [], 0
         for n, pages in zip(group_sizes, prefix_pages):
-            parts = 0
-            if n and pages:
-                splits = _prefix_splits(ctas, pages, slots)
-                keys = math.ceil(pages / 2)
-                cuts = [2 * (keys * s // splits) for s in range(splits)] + [pages]
-                parts = splits
+            keys = math.ceil(pages / 2)
+            cuts = [min(2 * (keys * s // self.splits), pages) for s in range(self.splits + 1)]
+            if pages:
                 for r0 in range(0, n, step):
-                    items += [[row + r0, min(step, n - r0), a, e - a, p, 0, 0, 0]
-                              for p, (a, e) in enumerate(zip(cuts, cuts[1:]))]
-            info += [[pages * PAGE if parts else 0, parts]] * n
-            self.parts = max(self.parts, parts)
+                    items += [[row + r0, min(step, n - r0), a, e - a] for a, e in zip(cuts, cuts[1:])]
+            info += [pages * PAGE] * n
             row += n
         self.items_n = len(items)
-        self.partials = self.rows * n_q * self.parts  # (row, head, part) results that a SpanWorkspace has to hold
-        host = torch.tensor(items or [[0] * _ITEM], dtype=_I32), torch.tensor(info or [[0, 0]], dtype=_I32)
+        self.partials = self.rows * n_q if items else 0  # (row, head) results that a SpanWorkspace has to hold
+        host = torch.tensor(items or [[0] * 4], dtype=_I32), torch.tensor(info or [0], dtype=_I32)
         if arena is not None:
-            self.items, self.row_info = (arena.empty(tuple(t.shape), _I32) for t in host)
+            self.items, self.row_prefix = (arena.empty(tuple(t.shape), _I32) for t in host)
             self.items.copy_(host[0])
-            self.row_info.copy_(host[1])
+            self.row_prefix.copy_(host[1])
         else:
             device = device or torch.device("cuda", torch.cuda.current_device())
-            self.items, self.row_info = (t.to(device) for t in host)
+            self.items, self.row_prefix = (t.to(device) for t in host)
 
 
 def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -263,12 +261,12 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if plan.items_n:
         g, rows = n_q // n_kv, blocks * n_kv * PAGE
         maps = core().make_tmaps_bf16([
-            (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g)),
-            (k_cache.data_ptr(), 128, rows, 256, PAGE), (v_cache.data_ptr(), 128, rows, 256, PAGE)])
+            (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0),
+            (k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0), (v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0)])
         _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (128 * plan.tiles + 64,), [
             maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
-            ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, plan.parts, blocks, scale * LOG2E],
-            TILE_SMEM[plan.tiles], _rt.raw_stream())
+            ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, blocks, scale * LOG2E],
+            TILE_SMEM[plan.tiles], _rt.raw_stream(), (plan.splits,))
     _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan)
     return out
 
@@ -295,7 +293,7 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
             ld = heads * 128
         if inner != 1 or ld % 8 or ld < heads * 128 or x.data_ptr() % 16:
             raise ValueError("q, k, v and out must be row-contiguous with 16-byte aligned rows that do not overlap")
-        maps.append((x.data_ptr(), heads * 128, t, ld * 2, TILE))
+        maps.append((x.data_ptr(), heads * 128, t, ld * 2, TILE, 0, 0))
     for x in (cu_seqlens, tile_seq, tile_start):
         if not (x.dtype is _I32 and x.dim() == 1 and x.is_contiguous()):
             raise ValueError("cu_seqlens and the tile tables must be contiguous int32")
