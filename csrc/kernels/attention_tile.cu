@@ -38,6 +38,8 @@
 //
 // Roles: warps [0, 4 QT) softmax and epilogue, then one TMA warp, one MMA warp.
 // No TMA multicast; every wait bounded (fb_common.cuh).
+#include <type_traits>
+
 #include "attn_tile.cuh"
 
 FB_DEFINE_STATUS
@@ -71,6 +73,36 @@ struct Smem {
 static_assert(sizeof(Smem<2>) + 1024 <= 226 * 1024, "host requests 226 KB of dynamic shared memory (2 tiles)");
 static_assert(sizeof(Smem<1>) + 1024 <= 98 * 1024, "host requests 98 KB of dynamic shared memory (1 tile)");
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x for x in [-inf, 16], one of POLY_OF pairs of scores: the special-function
+// unit gives 16 exponentials a clock and SM, as many as the two products of a tile
+// take time for; some on the FMA pipes bring the softmax below the products.
+// x = n + f, |f| <= 1/2; 2^f by the polynomial of degree 4 with the least relative
+// error (2.7e-6, found by linear programming; p is rounded to 2^-9 next). x below
+// -126 gives 2^-126 at least.
+constexpr int POLY_OF = 4;
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f);
+  const float2 t = __fadd2_rn(x, magic);  // the low bits are n
+  const float2 n = __fadd2_rn(t, unmagic);
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(0.00957010165f, 0.00957010165f);
+  p = __ffma2_rn(p, f, make_float2(0.0559178605f, 0.0559178605f));
+  p = __ffma2_rn(p, f, make_float2(0.240247448f, 0.240247448f));
+  p = __ffma2_rn(p, f, make_float2(0.693121815f, 0.693121815f));
+  p = __ffma2_rn(p, f, make_float2(0.999999261f, 0.999999261f));
+  p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return p;
+}
+
 // ---- thread-block clusters ----
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
@@ -103,6 +135,18 @@ __device__ __forceinline__ float2 load_remote2(uint32_t a) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
   return v;
+}
+
+// The softmax threads hold a row of scores: with two tiles they take registers
+// that the other warps do not need (65,536 / 384 threads = 168 at launch;
+// 256 x 208 + 128 x 88 = 384 x 168).
+template <int QT>
+__device__ __forceinline__ void take_registers() {
+  if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+}
+template <int QT>
+__device__ __forceinline__ void give_registers() {
+  if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
 
 // What the body needs of a CTA's work: n key tiles, tile i starting at key
@@ -145,6 +189,7 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     if (warp < 4 * QT) sm.ml(warp >> 2)[threadIdx.x & 127] = make_float2(-INFINITY, 0.f);
   } else if (warp == 4 * QT) {
     // ---------------- TMA producer ----------------
+    give_registers<QT>();
     if (lane == 0) {
       w.load_q(sm, &sm.q_full);
       int slot = 0;
@@ -177,70 +222,75 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     }
   } else if (warp == 4 * QT + 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      constexpr uint32_t id_qk = idesc_bf16<128, 128>();
-      constexpr uint32_t id_pv = idesc_bf16<128, 128>() | (1u << 16);  // B (V) MN-major
-      int kslot = 0, vslot = 1 % SLOTS;
-      uint32_t kphase = 0, vphase = 0;
-      auto next = [](int& s, uint32_t& ph) {
-        s += 2;
-        if (s >= SLOTS) {
-          s -= SLOTS;
-          ph ^= 1;
-        }
-      };
-      auto qk = [&](int t) {
-        const uint32_t qb = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
+    give_registers<QT>();
+    // The warp stays together: what the instructions take (descriptors, addresses)
+    // is then computed once for the warp, and one elected lane issues them.
+    constexpr uint32_t id_qk = idesc_bf16<128, 128>();
+    constexpr uint32_t id_pv = idesc_bf16<128, 128>() | (1u << 16);  // B (V) MN-major
+    const uint64_t q_desc = sdesc_sw128(smem_u32(sm.q[0])), k_desc = sdesc_sw128(smem_u32(sm.kv[0]));
+    const uint64_t v_desc = sdesc_mn_sw128(smem_u32(sm.kv[0]), HALF, 1024);
+    const bool issuer = elect_one();
+    int kslot = 0, vslot = 1 % SLOTS;
+    uint32_t kphase = 0, vphase = 0;
+    auto next = [](int& s, uint32_t& ph) {
+      s += 2;
+      if (s >= SLOTS) {
+        s -= SLOTS;
+        ph ^= 1;
+      }
+    };
+    auto qk = [&](int t) {
+      const uint64_t qd = q_desc + t * (TILE / 16), kd = k_desc + kslot * (TILE / 16);
+      if (issuer) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // K = 128 head dims, 16 per MMA
-          const uint32_t off = (k >> 2) * HALF + (k & 3) * 32;
-          mma_bf16(tmem + t * 128, sdesc_sw128(qb + off), sdesc_sw128(kb + off), id_qk, k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) / 16;
+          mma_bf16(tmem + t * 128, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
         }
         mma_commit(&sm.s_full[t]);
-      };
-      bool ok = mbar_wait(&sm.q_full, 0, FB_KERR_TIMEOUT_FULL) && mbar_wait(&sm.kv_full[0], 0, FB_KERR_TIMEOUT_FULL);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < QT; ++t) qk(t);
-        mma_commit(&sm.kv_empty[0]);
-        next(kslot, kphase);
       }
-      for (int i = 0; ok && i < n; ++i) {
-        ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
-#pragma unroll 1
-        for (int t = 0; ok && t < QT; ++t) {
-          if (!mbar_wait(&sm.p_full[t], i & 1, FB_KERR_TIMEOUT_TMEM)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t vb = smem_u32(sm.kv[vslot]);
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (issuer) mma_commit(bar);
+    };
+    bool ok = mbar_wait(&sm.q_full, 0, FB_KERR_TIMEOUT_FULL) && mbar_wait(&sm.kv_full[0], 0, FB_KERR_TIMEOUT_FULL);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+      for (int t = 0; t < QT; ++t) qk(t);
+      commit(&sm.kv_empty[0]);
+      next(kslot, kphase);
+    }
+    for (int i = 0; ok && i < n; ++i) {
+      ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
+      const uint64_t vd = v_desc + vslot * (TILE / 16);
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        ok = ok && mbar_wait(&sm.p_full[t], i & 1, FB_KERR_TIMEOUT_TMEM);
+        if (t == 0 && i + 1 < n) ok = ok && mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (issuer) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)  // K = 128 keys, 16 per MMA
-            mma_bf16_ts(tmem + (QT + t) * 128, tmem + t * 128 + k * 8, sdesc_mn_sw128(vb + k * 2048, HALF, 1024),
-                        id_pv, (i > 0 || k > 0) ? 1u : 0u);
-          if (t == QT - 1) mma_commit(&sm.kv_empty[vslot]);
-          if (i + 1 < n) {
-            if (t == 0 && !mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            qk(t);
-          } else {
-            mma_commit(&sm.o_full[t]);
-          }
+            mma_bf16_ts(tmem + (QT + t) * 128, tmem + t * 128 + k * 8, vd + k * (2048 / 16), id_pv,
+                        (i > 0 || k > 0) ? 1u : 0u);
         }
-        if (ok && i + 1 < n) {
-          mma_commit(&sm.kv_empty[kslot]);
-          next(kslot, kphase);
-        }
-        next(vslot, vphase);
+        if (t == QT - 1) commit(&sm.kv_empty[vslot]);
+        if (i + 1 < n) qk(t);
+        else commit(&sm.o_full[t]);
       }
-      if (!ok) sm.abort = 1;
+      if (ok && i + 1 < n) {
+        commit(&sm.kv_empty[kslot]);
+        next(kslot, kphase);
+      }
+      next(vslot, vphase);
     }
-  } else {
+    if (!ok) sm.abort = 1;
+  } else if (warp < 4 * QT) {
     // ---------------- softmax + epilogue ----------------
+    take_registers<QT>();
     const int t = warp >> 2;                         // query tile
     const int r = (warp & 3) * 32 + lane;            // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -263,7 +313,8 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
       for (int c = 0; c < 128; c += 32) tmem_ld32(t_s + c, sr + c);
       tmem_ld_wait();
       // Edge tiles: scores of keys that the row does not see become -inf.
-      if (__any_sync(0xffffffffu, k0 + BK - 1 > hi || (k0 < lo && k0 + BK > sinks))) {
+      const bool edge = __any_sync(0xffffffffu, k0 + BK - 1 > hi || (k0 < lo && k0 + BK > sinks));
+      if (edge) {
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
           const int b = k0 + c;
@@ -287,8 +338,9 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
       }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(sr[c]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+      for (int c = 0; c < 128; c += 2)
+        mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+      const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale_log2;
       const float m_new = mx > m_run + RESCALE_LOG2 || m_run == -INFINITY ? fmaxf(m_run, mx) : m_run;
       const float m_use = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = exp2f(m_run - m_use);  // 1 unless the max moved; 0 while nothing was seen
@@ -303,27 +355,40 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
           tmem_st32(t_o + c, o);
         }
       }
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 128; c += 64) {
+      // p = 2^(s scale - m)
+      float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const float2 scale2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m_use, -m_use);
+      auto half = [&](int h, auto poly) {
         uint32_t pk[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float p0 = exp2f(fmaf(__uint_as_float(sr[c + 2 * e]), scale_log2, -m_use));
-          const float p1 = exp2f(fmaf(__uint_as_float(sr[c + 2 * e + 1]), scale_log2, -m_use));
-          rs[(2 * e) & 3] += p0;
-          rs[(2 * e + 1) & 3] += p1;
-          const bf162 h = __floats2bfloat162_rn(p0, p1);
-          pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+          const int c = 64 * h + 2 * e;
+          float2 y = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, m2);
+          if (poly && QT == 2 && e % POLY_OF == POLY_OF - 1) {
+            y = exp2_poly(y);
+          } else {
+            y.x = exp2f(y.x);
+            y.y = exp2f(y.y);
+          }
+          rs[e & 1] = __fadd2_rn(rs[e & 1], y);
+          const bf162 b = __floats2bfloat162_rn(y.x, y.y);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&b);
         }
-        tmem_st32(t_s + c / 2, pk);
+        tmem_st32(t_s + 32 * h, pk);
+      };
+      if (edge) {  // exact zeros for what is masked
+        half(0, std::false_type());
+        half(1, std::false_type());
+      } else {
+        half(0, std::true_type());
+        half(1, std::true_type());
       }
       tmem_st_wait();
-      l_run = l_run * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-      m_run = m_new;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[t]);
+      l_run = l_run * alpha + ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y));
+      m_run = m_new;
     }
     for (int i = 0; ok && i < QT; ++i)  // of every tile: a store may reuse the ring
       if (i == t || Work::REUSES_RING) ok = mbar_wait(&sm.o_full[i], 0, FB_KERR_TIMEOUT_TMEM);
@@ -333,6 +398,8 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     } else {
       sm.abort = 1;
     }
+  } else {
+    give_registers<QT>();
   }
   w.finish(sm);
   tc_fence_before();
@@ -599,7 +666,7 @@ struct TileMaps {
 // rows. Grid: (query tiles of tile_seq / tile_start, Hq / QT). out [T, ld_o]
 // bf16, head h at columns h * 128; rows outside every prompt are not written.
 #define FB_WINDOW_PREFILL(QT, CTAS)                                                                               \
-  extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_window_prefill_q##QT(                      \
+  extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_window_prefill_q##QT(                      \
       const __grid_constant__ TileMaps maps, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,     \
       const int* tile_start, int Hq, int Hkv, int window, int sinks, float scale_log2) {                          \
     window_prefill<QT>(&maps.q, &maps.k, &maps.v, out, ld_o, cu_seqlens, tile_seq, tile_start, Hq, Hkv, window,   \
@@ -612,7 +679,7 @@ FB_WINDOW_PREFILL(2, 1)
 // 128] with boxes of one page. Grid: (items, Hkv), clusters of the items that
 // share their rows. The result of (row, head) is at index row * Hq + head.
 #define FB_PREFIX_ATTN(QT, CTAS)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(128 * QT + 64, CTAS) fb_prefix_attn_q##QT(                         \
+  extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_prefix_attn_q##QT(                         \
       const __grid_constant__ TileMaps maps, const PrefixItem* items, const int* block_tables, int max_blocks,    \
       const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks, float scale_log2) {      \
     prefix_attention<QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \

@@ -25,6 +25,7 @@ _SPAN, _TILE = "attention_span", "attention_tile"
 MAX_GROUP = 16
 SPAN_SMEM = 74 * 1024
 TILE_SMEM = {1: 98 * 1024, 2: 226 * 1024}
+TILE_THREADS = {1: 192, 2: 384}
 TILE = 128  # queries (and keys) of a tile
 MAX_CLUSTER = 8  # CTAs that share a prefix's pages between them
 _BF16, _I32 = torch.bfloat16, torch.int32
@@ -263,7 +264,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         maps = core().make_tmaps_bf16([
             (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0),
             (k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0), (v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0)])
-        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (128 * plan.tiles + 64,), [
+        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (TILE_THREADS[plan.tiles],), [
             maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
             ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, blocks, scale * LOG2E],
             TILE_SMEM[plan.tiles], _rt.raw_stream(), (plan.splits,))
@@ -304,7 +305,7 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     if not n_tiles or not t:
         return out
     qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
-    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (n_tiles, n_q // qt), (128 * qt + 64,), [
+    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (n_tiles, n_q // qt), (TILE_THREADS[qt],), [
         core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(),
         tile_start.data_ptr(), n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
     return out
