@@ -57,22 +57,37 @@ constexpr int TILE = 2 * HALF;       // 128 rows x 128 dims bf16
 constexpr float RESCALE_LOG2 = 8.f;  // lazy-rescale threshold
 constexpr int EVERY_KEY = 0x3fffffff;
 constexpr int MAX_CLUSTER = 8;
+constexpr int FEW = 32;  // keys of a tile of nothing but sinks
 
-template <int QT>
+// ROWS: of the output rows that each softmax warp stages for its stores (0: none).
+template <int QT_, int ROWS_>
 struct Smem {
-  static constexpr int SLOTS = QT == 2 ? 5 : 2;  // ring of K_0, V_0, K_1, V_1, ...
+  static constexpr int QT = QT_, ROWS = ROWS_;
+  static constexpr int SLOTS = QT == 1 ? 2 : ROWS ? 4 : 5;  // ring of K_0, V_0, K_1, V_1, ...
   uint8_t q[QT][TILE];
   uint8_t kv[SLOTS][TILE];
-  uint64_t q_full, kv_full[SLOTS], kv_empty[SLOTS];
+  uint8_t stage[4 * QT][ROWS ? ROWS * 256 : 16];
+  uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS];
   uint64_t s_full[QT], p_full[QT], o_full[QT];
   uint32_t tmem;
   int abort;
   // (max, sum) of each row for the cluster's join: in q's memory, when the products are done
   __device__ __forceinline__ float2* ml(int t) { return reinterpret_cast<float2*>(q[0]) + t * BQ; }
 };
-static_assert(sizeof(Smem<2>) + 1024 <= 226 * 1024, "host requests 226 KB of dynamic shared memory (2 tiles)");
-static_assert(sizeof(Smem<1>) + 1024 <= 98 * 1024, "host requests 98 KB of dynamic shared memory (1 tile)");
+using PrefixSmem1 = Smem<1, 0>;
+using PrefixSmem2 = Smem<2, 0>;
+using WindowSmem1 = Smem<1, 8>;
+using WindowSmem2 = Smem<2, 16>;
+static_assert(sizeof(PrefixSmem2) + 1024 <= 226 * 1024 && sizeof(WindowSmem2) + 1024 <= 226 * 1024,
+              "host requests 226 KB of dynamic shared memory (2 tiles)");
+static_assert(sizeof(PrefixSmem1) + 1024 <= 106 * 1024 && sizeof(WindowSmem1) + 1024 <= 106 * 1024,
+              "host requests 106 KB of dynamic shared memory (1 tile)");
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -87,8 +102,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // -126 gives 2^-126 at least.
 constexpr int POLY_OF = 4;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = max_nan(x.x, -126.f);
+  x.y = max_nan(x.y, -126.f);
   const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f);
   const float2 t = __fadd2_rn(x, magic);  // the low bits are n
   const float2 n = __fadd2_rn(t, unmagic);
@@ -149,16 +164,17 @@ __device__ __forceinline__ void give_registers() {
   if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
 
-// What the body needs of a CTA's work: n key tiles, tile i starting at key
-// position key0(i); loads; and each row's visible keys
+// What the body needs of a CTA's work: its items one after another (next() in
+// every role); an item's n key tiles, tile i starting at key position key0(i),
+// tile 0 of FEW keys only if `few`; loads; and each row's visible keys
 // {kp : kp <= hi and (kp >= lo or kp < sinks)}.
-template <int QT, class Work>
-__device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, float scale_log2) {
-  constexpr int SLOTS = Smem<QT>::SLOTS;
+template <class Work, class Smem>
+__device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log2) {
+  constexpr int QT = Smem::QT, SLOTS = Smem::SLOTS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = w.n;
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&sm.kv_full[s], 1);
       mbar_init(&sm.kv_empty[s], 1);
@@ -184,33 +200,39 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
   pdl_trigger();  // not before: a dependent's CTA must not take TMEM that this one has yet to allocate
   const uint32_t tmem = sm.tmem;  // S_t at columns 128 t, O_t at 128 (QT + t)
 
-  if (n == 0) {
-    // nothing for this CTA of a cluster (w.finish below still counts on it)
-    if (warp < 4 * QT) sm.ml(warp >> 2)[threadIdx.x & 127] = make_float2(-INFINITY, 0.f);
-  } else if (warp == 4 * QT) {
+  if (warp == 4 * QT) {
     // ---------------- TMA producer ----------------
     give_registers<QT>();
     if (lane == 0) {
-      w.load_q(sm, &sm.q_full);
-      int slot = 0;
+      int slot = 0, items = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int i = 0; ok && i < n; ++i) {
+      for (; ok && w.next(); ++items) {
+        for (int i = 0; ok && i < w.n; ++i) {
 #pragma unroll 1
-        for (int v = 0; v < 2; ++v) {
-          if (!mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
-            sm.abort = 1;
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&sm.kv_full[slot], TILE);
-          w.load_kv(sm.kv[slot], &sm.kv_full[slot], i, v);
-          if (++slot == SLOTS) {
-            slot = 0;
-            phase ^= 1;
+          for (int v = 0; v < 2; ++v) {
+            // q comes behind the first K, whose slot is free before the last item's q is
+            if (i == 0 && v == 1) {
+              if (!mbar_wait(&sm.q_empty, (items & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
+                ok = false;
+                break;
+              }
+              w.load_q(sm, &sm.q_full);
+            }
+            if (!mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&sm.kv_full[slot], TILE);
+            w.load_kv(sm.kv[slot], &sm.kv_full[slot], i, v);
+            if (++slot == SLOTS) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
       }
+      if (!ok) sm.abort = 1;
       // Drain: every copy has landed and been consumed before the CTA leaves.
       for (int s = 0; ok && s < SLOTS; ++s) {
         mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
@@ -225,7 +247,7 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     give_registers<QT>();
     // The warp stays together: what the instructions take (descriptors, addresses)
     // is then computed once for the warp, and one elected lane issues them.
-    constexpr uint32_t id_qk = idesc_bf16<128, 128>();
+    constexpr uint32_t id_qk = idesc_bf16<128, 128>(), id_qk_few = idesc_bf16<128, FEW>();
     constexpr uint32_t id_pv = idesc_bf16<128, 128>() | (1u << 16);  // B (V) MN-major
     const uint64_t q_desc = sdesc_sw128(smem_u32(sm.q[0])), k_desc = sdesc_sw128(smem_u32(sm.kv[0]));
     const uint64_t v_desc = sdesc_mn_sw128(smem_u32(sm.kv[0]), HALF, 1024);
@@ -239,13 +261,13 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
         ph ^= 1;
       }
     };
-    auto qk = [&](int t) {
+    auto qk = [&](int t, uint32_t id) {
       const uint64_t qd = q_desc + t * (TILE / 16), kd = k_desc + kslot * (TILE / 16);
       if (issuer) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {  // K = 128 head dims, 16 per MMA
           const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) / 16;
-          mma_bf16(tmem + t * 128, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
+          mma_bf16(tmem + t * 128, qd + off, kd + off, id, k > 0 ? 1u : 0u);
         }
         mma_commit(&sm.s_full[t]);
       }
@@ -253,39 +275,50 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     auto commit = [&](uint64_t* bar) {
       if (issuer) mma_commit(bar);
     };
-    bool ok = mbar_wait(&sm.q_full, 0, FB_KERR_TIMEOUT_FULL) && mbar_wait(&sm.kv_full[0], 0, FB_KERR_TIMEOUT_FULL);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+    uint32_t tiles = 0, items = 0;  // key tiles and items so far
+    bool ok = true;
+    for (; ok && w.next(); ++items) {
+      const int n = w.n;
+      if (n == 0) continue;
+      ok = mbar_wait(&sm.q_full, items & 1, FB_KERR_TIMEOUT_FULL) &&
+           mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < QT; ++t) qk(t);
-      commit(&sm.kv_empty[0]);
+      // S and P of the last item are done with: its last P V is issued, behind its last softmax
+      for (int t = 0; t < QT; ++t) qk(t, w.few ? id_qk_few : id_qk);
+      commit(&sm.kv_empty[kslot]);
+      if (n == 1) commit(&sm.q_empty);
       next(kslot, kphase);
-    }
-    for (int i = 0; ok && i < n; ++i) {
-      ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
-      const uint64_t vd = v_desc + vslot * (TILE / 16);
+      for (int i = 0; ok && i < n; ++i, ++tiles) {
+        ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
+        const uint64_t vd = v_desc + vslot * (TILE / 16);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        ok = ok && mbar_wait(&sm.p_full[t], i & 1, FB_KERR_TIMEOUT_TMEM);
-        if (t == 0 && i + 1 < n) ok = ok && mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (issuer) {
+        for (int t = 0; t < QT; ++t) {
+          ok = ok && mbar_wait(&sm.p_full[t], tiles & 1, FB_KERR_TIMEOUT_TMEM);
+          if (t == 0 && i + 1 < n) ok = ok && mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (issuer) {
+            const int steps = i == 0 && w.few ? FEW / 16 : 8;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)  // K = 128 keys, 16 per MMA
-            mma_bf16_ts(tmem + (QT + t) * 128, tmem + t * 128 + k * 8, vd + k * (2048 / 16), id_pv,
-                        (i > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < 8; ++k)  // K = 128 keys, 16 per MMA
+              if (k < steps)
+                mma_bf16_ts(tmem + (QT + t) * 128, tmem + t * 128 + k * 8, vd + k * (2048 / 16), id_pv,
+                            (i > 0 || k > 0) ? 1u : 0u);
+          }
+          if (t == QT - 1) commit(&sm.kv_empty[vslot]);
+          if (i + 1 < n) qk(t, id_qk);
+          else commit(&sm.o_full[t]);
         }
-        if (t == QT - 1) commit(&sm.kv_empty[vslot]);
-        if (i + 1 < n) qk(t);
-        else commit(&sm.o_full[t]);
+        if (ok && i + 1 < n) {
+          commit(&sm.kv_empty[kslot]);
+          if (i + 2 == n) commit(&sm.q_empty);
+          next(kslot, kphase);
+        }
+        next(vslot, vphase);
       }
-      if (ok && i + 1 < n) {
-        commit(&sm.kv_empty[kslot]);
-        next(kslot, kphase);
-      }
-      next(vslot, vphase);
     }
     if (!ok) sm.abort = 1;
   } else if (warp < 4 * QT) {
@@ -295,109 +328,144 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
     const int r = (warp & 3) * 32 + lane;            // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t * 128 + lane_base, t_o = tmem + (QT + t) * 128 + lane_base;
-    int hi, lo;
-    w.row_range(t, r, hi, lo);
-    const int sinks = w.sinks;
-    float m_run = -INFINITY, l_run = 0.f;
+    uint32_t tiles = 0, items = 0;
     bool ok = true;
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int k0 = w.key0(i);
-      if (!mbar_wait(&sm.s_full[t], i & 1, FB_KERR_TIMEOUT_TMEM)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t sr[128];
-#pragma unroll
-      for (int c = 0; c < 128; c += 32) tmem_ld32(t_s + c, sr + c);
-      tmem_ld_wait();
-      // Edge tiles: scores of keys that the row does not see become -inf.
-      const bool edge = __any_sync(0xffffffffu, k0 + BK - 1 > hi || (k0 < lo && k0 + BK > sinks));
-      if (edge) {
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          const int b = k0 + c;
-          const uint32_t seen = bits_below(hi + 1 - b) & (~bits_below(lo - b) | bits_below(sinks - b));
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen >> e) & 1u)) sr[c + e] = 0xff800000u;
-        }
-      }
-      if (t == 0 && w.zero_row(i, r)) {
-        // A key row behind the prompt's end holds another prompt's values or
-        // nothing at all, and 0 * NaN = NaN: its V row is zeroed once the copy
-        // has landed (tile 0's P V runs first, so once is enough).
-        const int slot = (2 * i + 1) % SLOTS;
-        if (!mbar_wait(&sm.kv_full[slot], ((2 * i + 1) / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
-        uint8_t* vrow = sm.kv[slot] + r * 128;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async();
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 128; c += 2)
-        mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-      const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale_log2;
-      const float m_new = mx > m_run + RESCALE_LOG2 || m_run == -INFINITY ? fmaxf(m_run, mx) : m_run;
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m_run - m_use);  // 1 unless the max moved; 0 while nothing was seen
-      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(t_o + c, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(t_o + c, o);
-        }
-      }
-      // p = 2^(s scale - m)
-      float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const float2 scale2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m_use, -m_use);
-      auto half = [&](int h, auto poly) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int c = 64 * h + 2 * e;
-          float2 y = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, m2);
-          if (poly && QT == 2 && e % POLY_OF == POLY_OF - 1) {
-            y = exp2_poly(y);
-          } else {
-            y.x = exp2f(y.x);
-            y.y = exp2f(y.y);
-          }
-          rs[e & 1] = __fadd2_rn(rs[e & 1], y);
-          const bf162 b = __floats2bfloat162_rn(y.x, y.y);
-          pk[e] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        tmem_st32(t_s + 32 * h, pk);
+    for (; ok && w.next(); ++items) {
+      int hi, lo;
+      w.row_range(t, r, hi, lo);
+      const int sinks = w.sinks, n = w.n;
+      float m_run = -INFINITY, l_run = 0.f;
+      // The keys k0 .. k0 + 31 that the row sees, as bits.
+      auto seen = [&](int k0) {
+        return bits_below(hi + 1 - k0) & (~bits_below(lo - k0) | bits_below(sinks - k0));
       };
-      if (edge) {  // exact zeros for what is masked
-        half(0, std::false_type());
-        half(1, std::false_type());
-      } else {
-        half(0, std::true_type());
-        half(1, std::true_type());
+#pragma unroll 1
+      for (int i = 0; i < n; ++i, ++tiles) {
+        const int k0 = w.key0(i);
+        if (!mbar_wait(&sm.s_full[t], tiles & 1, FB_KERR_TIMEOUT_TMEM)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (i == 0 && w.few) {
+          // A few sinks far before the window: a tile of FEW keys.
+          uint32_t sr[FEW], pk[FEW / 2];
+          tmem_ld32(t_s, sr);
+          tmem_ld_wait();
+          const uint32_t bits = seen(k0);
+#pragma unroll
+          for (int e = 0; e < FEW; ++e) {
+            if (!((bits >> e) & 1u)) sr[e] = 0xff800000u;
+            m_run = fmaxf(m_run, __uint_as_float(sr[e]) * scale_log2);
+          }
+          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+          for (int e = 0; e < FEW; e += 2) {
+            const float p0 = exp2f(fmaf(__uint_as_float(sr[e]), scale_log2, -m_use));
+            const float p1 = exp2f(fmaf(__uint_as_float(sr[e + 1]), scale_log2, -m_use));
+            l_run += p0 + p1;
+            const bf162 b = __floats2bfloat162_rn(p0, p1);
+            pk[e / 2] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          tmem_st16(t_s, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[t]);
+          continue;
+        }
+        uint32_t sr[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(t_s + c, sr + c);
+        tmem_ld_wait();
+        // Edge tiles: scores of keys that the row does not see become -inf.
+        const bool edge = __any_sync(0xffffffffu, k0 + BK - 1 > hi || (k0 < lo && k0 + BK > sinks));
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) {
+            const uint32_t bits = seen(k0 + c);
+            if (!__all_sync(0xffffffffu, bits == ~0u)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) sr[c + e] = 0xff800000u;
+            }
+          }
+        }
+        if (t == 0 && w.zero_row(i, r)) {
+          // A key row behind the prompt's end holds another prompt's values or
+          // nothing at all, and 0 * NaN = NaN: its V row is zeroed once the copy
+          // has landed (tile 0's P V runs first, so once is enough).
+          const uint32_t at = 2 * tiles + 1, slot = at % SLOTS;
+          if (!mbar_wait(&sm.kv_full[slot], (at / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
+          uint8_t* vrow = sm.kv[slot] + r * 128;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 128; c += 2)
+          mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale_log2;
+        const float m_new = mx > m_run + RESCALE_LOG2 || m_run == -INFINITY ? fmaxf(m_run, mx) : m_run;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f(m_run - m_use);  // 1 unless the max moved; 0 while nothing was seen
+        if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(t_o + c, o);
+          }
+        }
+        // p = 2^(s scale - m)
+        float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 scale2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m_use, -m_use);
+        auto half = [&](int h, auto poly) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int c = 64 * h + 2 * e;
+            float2 y = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, m2);
+            if (poly && QT == 2 && e % POLY_OF == POLY_OF - 1) {
+              y = exp2_poly(y);
+            } else {
+              y.x = exp2f(y.x);
+              y.y = exp2f(y.y);
+            }
+            rs[e & 1] = __fadd2_rn(rs[e & 1], y);
+            const bf162 b = __floats2bfloat162_rn(y.x, y.y);
+            pk[e] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          tmem_st32(t_s + 32 * h, pk);
+        };
+        if (edge) {  // exact zeros for what is masked
+          half(0, std::false_type());
+          half(1, std::false_type());
+        } else {
+          half(0, std::true_type());
+          half(1, std::true_type());
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[t]);
+        l_run = l_run * alpha + ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y));
+        m_run = m_new;
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full[t]);
-      l_run = l_run * alpha + ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y));
-      m_run = m_new;
+      for (int i = 0; ok && n > 0 && i < QT; ++i)  // of every tile: a store may reuse the ring
+        if (i == t || Work::REUSES_RING) ok = mbar_wait(&sm.o_full[i], items & 1, FB_KERR_TIMEOUT_TMEM);
+      if (ok) {
+        tc_fence_after();
+        w.store(sm, t, r, t_o, m_run, l_run);
+      }
     }
-    for (int i = 0; ok && i < QT; ++i)  // of every tile: a store may reuse the ring
-      if (i == t || Work::REUSES_RING) ok = mbar_wait(&sm.o_full[i], 0, FB_KERR_TIMEOUT_TMEM);
-    if (ok) {
-      tc_fence_after();
-      w.store(sm, t, r, t_o, m_run, l_run);
-    } else {
-      sm.abort = 1;
-    }
+    if (!ok) sm.abort = 1;
   } else {
     give_registers<QT>();
   }
@@ -408,26 +476,87 @@ __device__ __forceinline__ void tile_attention(const Work& w, Smem<QT>& sm, floa
   if (warp == 4 * QT + 1) tmem_dealloc(tmem, QT * 256);
 }
 
-template <int QT>
-__device__ __forceinline__ Smem<QT>& tile_smem() {
+template <class Smem>
+__device__ __forceinline__ Smem& tile_smem() {
   extern __shared__ uint8_t smem_raw[];
-  return *reinterpret_cast<Smem<QT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  return *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 }
 
 // ---- windowed causal prefill -----------------------------------------------------------
-// Key tiles of the query tile [qp0, qp0 + 128): those of the sinks, then those
-// of the window, at multiples of 128 of the prompt.
-template <int QT>
+// An item is a query tile [qp0, qp0 + 128) of a prompt for QT heads of one KV
+// head. Its key tiles: those of the sinks, then those of the window, at multiples
+// of 128 of the prompt. The grid is persistent: a prompt tile has few key tiles,
+// and the next item's copies and first product run during this one's end.
+template <class Smem>
 struct WindowWork {
+  static constexpr int QT = Smem::QT;
   const CUtensorMap *tmQ, *tmK, *tmV;
   bf16* out;
-  int ld_o, head0, kvh, s0, s1, qp0, window;
-  int n, n_sink, first, sinks;
+  const int *cu_seqlens, *tile_seq, *tile_start;
+  int ld_o, n_tiles, heads, group, window, all_sinks;
+  // Items go tile by tile, head by head: one of `tile` and `head` is next. What
+  // its tables say is read two items ahead (the tile's prompt), then one (where
+  // that begins and ends), so that nothing waits for them.
+  int tile, head, step_tile, step_head;
+  int seq2, start2, s0_1, s1_1, start1, tile1, head1;
+  int head0, kvh, s0, s1, qp0, n, n_sink, first, sinks;
+  bool few;
 
+  __device__ __forceinline__ void advance() {
+    s0_1 = s1_1 = 0;
+    start1 = start2;
+    tile1 = tile;
+    head1 = head;
+    if (tile1 < n_tiles) {
+      s0_1 = cu_seqlens[seq2];
+      s1_1 = cu_seqlens[seq2 + 1];
+    }
+    tile += step_tile;
+    head += step_head;
+    if (head >= heads) {
+      head -= heads;
+      ++tile;
+    }
+    if (tile < n_tiles) {
+      seq2 = tile_seq[tile];
+      start2 = tile_start[tile];
+    }
+  }
+  __device__ __forceinline__ void start() {
+    tile = blockIdx.x / heads;
+    head = blockIdx.x % heads;
+    step_tile = gridDim.x / heads;
+    step_head = gridDim.x % heads;
+    if (tile < n_tiles) {
+      seq2 = tile_seq[tile];
+      start2 = tile_start[tile];
+    }
+    advance();
+  }
+  __device__ __forceinline__ bool next() {
+    for (; tile1 < n_tiles; advance()) {
+      s0 = s0_1;
+      s1 = s1_1;
+      qp0 = start1;
+      const int end = min(qp0 + BQ, s1 - s0);  // queries and keys of this tile end here
+      if (qp0 < 0 || qp0 >= end) continue;     // a tile table that does not match cu_seqlens
+      head0 = head1 * QT;
+      kvh = head0 / group;
+      const int last = (end - 1) / BK, in_window = max(qp0 - window + 1, 0) / BK;
+      sinks = min(all_sinks, end);
+      n_sink = min((sinks + BK - 1) / BK, last + 1);
+      first = max(in_window, n_sink);
+      n = n_sink + last + 1 - first;
+      few = n_sink == 1 && sinks <= FEW && in_window > 0;
+      advance();
+      return true;
+    }
+    return false;
+  }
   __device__ __forceinline__ int key0(int i) const { return (i < n_sink ? i : i - n_sink + first) * BK; }
   __device__ __forceinline__ bool zero_row(int i, int r) const { return key0(i) + r >= s1 - s0; }
-  __device__ __forceinline__ void clear_q(Smem<QT>&) const {}
-  __device__ __forceinline__ void load_q(Smem<QT>& sm, uint64_t* bar) const {
+  __device__ __forceinline__ void clear_q(Smem&) const {}
+  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar) const {
     mbar_arrive_expect_tx(bar, QT * TILE);
     for (int t = 0; t < QT; ++t)
       for (int h = 0; h < 2; ++h) tma_load_2d(sm.q[t] + h * HALF, tmQ, bar, (head0 + t) * D + h * 64, s0 + qp0);
@@ -442,61 +571,76 @@ struct WindowWork {
     lo = qpos - window + 1;
   }
   static constexpr bool REUSES_RING = false;
-  __device__ __forceinline__ void finish(Smem<QT>&) const {}
-  __device__ __forceinline__ void store(Smem<QT>&, int t, int r, uint32_t t_o, float, float l) const {
+  __device__ __forceinline__ void finish(Smem&) const {}
+  // Rows go through shared memory, 16-byte chunks swizzled by the row, so that a
+  // store instruction writes two whole rows of the head: straight from a row per
+  // thread it would touch 32 lines, and the stores of a tile took as long as two
+  // key tiles.
+  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float, float l) const {
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const bool live = s0 + qp0 + r < s1;
-    bf16* row = out + static_cast<size_t>(s0 + qp0 + r) * ld_o + (head0 + t) * D;
-#pragma unroll 1
+    const int lane = r & 31, row0 = s0 + qp0 + (r & ~31);
+    uint4 packed[16];
+#pragma unroll
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
       tmem_ld32(t_o + c, o);
       tmem_ld_wait();
-      if (live) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float f[8];
+      for (int e = 0; e < 32; e += 8) {
+        float f[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[e + x]) * inv;
-          *reinterpret_cast<uint4*>(row + c + e) = pack8(f);
-        }
+        for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[e + x]) * inv;
+        packed[(c + e) / 8] = pack8(f);
+      }
+    }
+    uint8_t* stage = sm.stage[t * 4 + (r >> 5)];
+#pragma unroll 1
+    for (int p = 0; p < 32; p += Smem::ROWS) {
+      __syncwarp();
+      if (lane >= p && lane < p + Smem::ROWS) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          *reinterpret_cast<uint4*>(stage + (lane - p) * 256 + ((e ^ (lane & 15)) << 4)) = packed[e];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < Smem::ROWS / 2; ++e) {
+        const int row = 2 * e + (lane >> 4), chunk = lane & 15;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 256 + ((chunk ^ ((row + p) & 15)) << 4));
+        if (row0 + p + row < s1)
+          *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + p + row) * ld_o + (head0 + t) * D + chunk * 8) = v;
       }
     }
   }
 };
 
-template <int QT>
+template <class Smem>
 __device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV,
                                                bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,
-                                               const int* tile_start, int Hq, int Hkv, int window, int sinks,
-                                               float scale_log2) {
+                                               const int* tile_start, int n_tiles, int Hq, int Hkv, int window,
+                                               int sinks, float scale_log2) {
   pdl_wait();
-  WindowWork<QT> w;
+  WindowWork<Smem> w;
   w.tmQ = tmQ;
   w.tmK = tmK;
   w.tmV = tmV;
   w.out = out;
   w.ld_o = ld_o;
-  w.head0 = blockIdx.y * QT;  // QT heads of one KV head
-  w.kvh = w.head0 / (Hq / Hkv);
+  w.cu_seqlens = cu_seqlens;
+  w.tile_seq = tile_seq;
+  w.tile_start = tile_start;
+  w.n_tiles = n_tiles;
+  w.heads = Hq / Smem::QT;
+  w.group = Hq / Hkv;
   w.window = window;
-  const int seq = tile_seq[blockIdx.x];
-  w.s0 = cu_seqlens[seq];
-  w.s1 = cu_seqlens[seq + 1];
-  w.qp0 = tile_start[blockIdx.x];
-  const int end = min(w.qp0 + BQ, w.s1 - w.s0);  // queries and keys of this tile end here
-  if (w.qp0 < 0 || w.qp0 >= end) return;         // a tile table that does not match cu_seqlens
-  const int last = (end - 1) / BK;
-  w.sinks = min(sinks, end);
-  w.n_sink = min((w.sinks + BK - 1) / BK, last + 1);
-  w.first = max(max(w.qp0 - window + 1, 0) / BK, w.n_sink);
-  w.n = w.n_sink + last + 1 - w.first;
+  w.all_sinks = sinks;
+  w.start();
   if (threadIdx.x == 0) {
     tma_prefetch_desc(tmQ);
     tma_prefetch_desc(tmK);
     tma_prefetch_desc(tmV);
   }
-  tile_attention<QT>(w, tile_smem<QT>(), scale_log2);
+  tile_attention(w, tile_smem<Smem>(), scale_log2);
 }
 
 // ---- shared prefix of a decode batch ---------------------------------------------------
@@ -509,20 +653,28 @@ struct PrefixItem {
   int row0, rows, page0, pages;
 };
 
-template <int QT>
+template <class Smem>
 struct PrefixWork {
+  static constexpr int QT = Smem::QT;
   const CUtensorMap *tmQ, *tmK, *tmV;
   const int *pages, *seq_lens;
   float *o_part, *ml_part;
   PrefixItem it;
   int kvh, G, nb, Hq, Hkv, blocks;
   int n, sinks;
+  static constexpr bool few = false;
+  bool more = true;  // a CTA has one item (of no pages, maybe)
+  __device__ __forceinline__ bool next() {
+    const bool had = more;
+    more = false;
+    return had;
+  }
 
   __device__ __forceinline__ int key0(int i) const { return it.page0 * PAGE + i * BK; }
   __device__ __forceinline__ bool zero_row(int, int) const { return false; }
   // Rows that no head and sequence uses hold zeros and see every key: what
   // they compute is finite and dropped, and keeps no warp on the masked path.
-  __device__ __forceinline__ void clear_q(Smem<QT>& sm) const {
+  __device__ __forceinline__ void clear_q(Smem& sm) const {
     const int rows = 128 - G * nb;
     for (int e = threadIdx.x; e < QT * 2 * rows * 8; e += blockDim.x) {
       const int half = e / (rows * 8);  // tile * 2 + dim half
@@ -530,7 +682,7 @@ struct PrefixWork {
           make_uint4(0, 0, 0, 0);
     }
   }
-  __device__ __forceinline__ void load_q(Smem<QT>& sm, uint64_t* bar) const {
+  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar) const {
     mbar_arrive_expect_tx(bar, QT * 2 * G * nb * 128);
     for (int t = 0; t < QT; ++t)
       for (int g = 0; g < G; ++g)
@@ -565,11 +717,12 @@ struct PrefixWork {
   }
   static constexpr bool REUSES_RING = true;
   // O rows of the tiles in the ring's memory, 16-byte chunks swizzled by the row.
-  __device__ __forceinline__ static uint32_t o_at(Smem<QT>& sm, int t, int r, int chunk) {
+  __device__ __forceinline__ static uint32_t o_at(Smem& sm, int t, int r, int chunk) {
     return smem_u32(sm.kv[0]) + (t * BQ + r) * (D * 4) + ((chunk ^ (r & 31)) << 4);
   }
-  __device__ __forceinline__ void store(Smem<QT>& sm, int t, int r, uint32_t t_o, float m, float l) const {
+  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float m, float l) const {
     sm.ml(t)[r] = make_float2(m, l);
+    if (n == 0) return;  // O is nothing
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
@@ -584,7 +737,7 @@ struct PrefixWork {
   }
   // The cluster's CTAs have the same rows: a warp joins one row at a time, of
   // the rows that fall to its CTA.
-  __device__ __forceinline__ void finish(Smem<QT>& sm) const {
+  __device__ __forceinline__ void finish(Smem& sm) const {
     cluster_sync();
     const int size = cluster_size(), warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     for (int i = cluster_rank() * warps + (threadIdx.x >> 5); i < QT * BQ; i += size * warps) {
@@ -623,14 +776,14 @@ struct PrefixWork {
   }
 };
 
-template <int QT>
+template <class Smem>
 __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const CUtensorMap* tmK,
                                                  const CUtensorMap* tmV, const PrefixItem* items,
                                                  const int* block_tables, int max_blocks, const int* seq_lens,
                                                  float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks,
                                                  float scale_log2) {
   pdl_wait();
-  PrefixWork<QT> w;
+  PrefixWork<Smem> w;
   w.it = items[blockIdx.x];
   w.tmQ = tmQ;
   w.tmK = tmK;
@@ -652,7 +805,7 @@ __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const C
     tma_prefetch_desc(tmK);
     tma_prefetch_desc(tmV);
   }
-  tile_attention<QT>(w, tile_smem<QT>(), scale_log2);
+  tile_attention(w, tile_smem<Smem>(), scale_log2);
 }
 
 }  // namespace
@@ -663,14 +816,13 @@ struct TileMaps {
 };
 
 // q [T, Hq * 128], k, v [T, Hkv * 128]: maps over the packed rows, boxes of 128
-// rows. Grid: (query tiles of tile_seq / tile_start, Hq / QT). out [T, ld_o]
-// bf16, head h at columns h * 128; rows outside every prompt are not written.
+// rows. n_tiles query tiles of tile_seq / tile_start. out [T, ld_o] bf16, head h at columns h * 128; rows outside every prompt are not written.
 #define FB_WINDOW_PREFILL(QT, CTAS)                                                                               \
   extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_window_prefill_q##QT(                      \
       const __grid_constant__ TileMaps maps, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,     \
-      const int* tile_start, int Hq, int Hkv, int window, int sinks, float scale_log2) {                          \
-    window_prefill<QT>(&maps.q, &maps.k, &maps.v, out, ld_o, cu_seqlens, tile_seq, tile_start, Hq, Hkv, window,   \
-                       sinks, scale_log2);                                                                        \
+      const int* tile_start, int n_tiles, int Hq, int Hkv, int window, int sinks, float scale_log2) {             \
+    window_prefill<WindowSmem##QT>(&maps.q, &maps.k, &maps.v, out, ld_o, cu_seqlens, tile_seq, tile_start, n_tiles, Hq, Hkv,  \
+                       window, sinks, scale_log2);                                                                        \
   }
 FB_WINDOW_PREFILL(1, 2)
 FB_WINDOW_PREFILL(2, 1)
@@ -682,7 +834,7 @@ FB_WINDOW_PREFILL(2, 1)
   extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_prefix_attn_q##QT(                         \
       const __grid_constant__ TileMaps maps, const PrefixItem* items, const int* block_tables, int max_blocks,    \
       const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks, float scale_log2) {      \
-    prefix_attention<QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \
+    prefix_attention<PrefixSmem##QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \
                          G, Hq, Hkv, blocks, scale_log2);                                                         \
   }
 FB_PREFIX_ATTN(1, 2)

@@ -85,12 +85,15 @@ def pdl_active() -> bool:
 
 
 def launch(image: str, name: str, grid, block, args, smem: int = 0, stream: int | None = None,
-           cluster=()) -> None:
+           cluster=(), after_own: bool = False) -> None:
+    """``after_own``: the launch right before it on this stream is one of the
+    same op; this kernel may be set up while that one runs (it waits for it
+    before it reads anything, as every kernel of ``PDL_IMAGES`` does)."""
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
     fn = function(image, name, smem)
     core().launch(fn, tuple(grid), tuple(block), smem, stream, args, tuple(cluster),
-                  pdl_active() and image in PDL_IMAGES)
+                  (after_own and PDL_ENABLED) or (pdl_active() and image in PDL_IMAGES))
 
 
 def raw_stream() -> int:

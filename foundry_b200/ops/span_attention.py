@@ -24,7 +24,7 @@ from .attention import LOG2E, PAGE
 _SPAN, _TILE = "attention_span", "attention_tile"
 MAX_GROUP = 16
 SPAN_SMEM = 74 * 1024
-TILE_SMEM = {1: 98 * 1024, 2: 226 * 1024}
+TILE_SMEM = {1: 106 * 1024, 2: 226 * 1024}
 TILE_THREADS = {1: 192, 2: 384}
 TILE = 128  # queries (and keys) of a tile
 MAX_CLUSTER = 8  # CTAs that share a prefix's pages between them
@@ -143,7 +143,7 @@ class SpanWorkspace:
 
 
 def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, dims, window: int, sinks: int,
-          scale: float, plan: "PrefixPlan | None") -> None:
+          scale: float, plan: "PrefixPlan | None" = None) -> None:
     b, n_q, n_kv, blocks, max_blocks = dims
     g = n_q // n_kv
     k, v, rows = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE
@@ -158,7 +158,7 @@ def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, d
                (min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)),), (192,), [
         maps, block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv,
         g, window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(),
-        ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream())
+        ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream(), (), plan is not None)
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -175,7 +175,7 @@ def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     _check_window(window, sinks)
     scale = _check_scale(scale)
     if dims[0]:
-        _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, window, sinks, scale, None)
+        _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, window, sinks, scale)
     return out
 
 
@@ -268,7 +268,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
             ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, blocks, scale * LOG2E],
             TILE_SMEM[plan.tiles], _rt.raw_stream(), (plan.splits,))
-    _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan)
+    _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan if plan.items_n else None)
     return out
 
 
@@ -305,7 +305,8 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     if not n_tiles or not t:
         return out
     qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
-    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (n_tiles, n_q // qt), (TILE_THREADS[qt],), [
+    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (min(n_tiles * (n_q // qt), _rt.sm_count() * (3 - qt)),),
+               (TILE_THREADS[qt],), [
         core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(),
-        tile_start.data_ptr(), n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
+        tile_start.data_ptr(), n_tiles, n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
     return out
