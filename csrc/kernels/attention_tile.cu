@@ -36,7 +36,8 @@
 // p is rounded to bf16 for the second product (relative 2^-9 per term, with
 // random signs), the sum l and both products accumulate in fp32.
 //
-// Roles: warps [0, 4 QT) softmax and epilogue, then one TMA warp, one MMA warp.
+// Roles: warps [0, 4 QT) softmax (and epilogue, but for the two-tile prefill, which
+// has four warps for that), then one TMA warp, one MMA warp.
 // No TMA multicast; every wait bounded (fb_common.cuh).
 #include <type_traits>
 
@@ -59,16 +60,17 @@ constexpr int EVERY_KEY = 0x3fffffff;
 constexpr int MAX_CLUSTER = 8;
 constexpr int FEW = 32;  // keys of a tile of nothing but sinks
 
-// ROWS: of the output rows that each softmax warp stages for its stores (0: none).
-template <int QT_, int ROWS_>
+// STAGE: bytes per row of the output that a warp stages for its stores (0: none).
+template <int QT_, int STAGE_>
 struct Smem {
-  static constexpr int QT = QT_, ROWS = ROWS_;
-  static constexpr int SLOTS = QT == 1 ? 2 : ROWS ? 4 : 5;  // ring of K_0, V_0, K_1, V_1, ...
+  static constexpr int QT = QT_, STAGE = STAGE_;
+  static constexpr int SLOTS = QT == 1 ? 2 : STAGE ? 4 : 5;  // ring of K_0, V_0, K_1, V_1, ...
   uint8_t q[QT][TILE];
   uint8_t kv[SLOTS][TILE];
-  uint8_t stage[4 * QT][ROWS ? ROWS * 256 : 16];
-  uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS];
-  uint64_t s_full[QT], p_full[QT], o_full[QT];
+  uint8_t stage[4][STAGE ? 32 * STAGE : 16];
+  float l[QT][STAGE && QT == 2 ? BQ : 1];  // the rows' sums for the epilogue
+  uint64_t q_full[QT], q_empty[QT], kv_full[SLOTS], kv_empty[SLOTS];
+  uint64_t s_full[QT], p_full[QT], o_full[QT], l_full[QT], o_empty[QT];
   uint32_t tmem;
   int abort;
   // (max, sum) of each row for the cluster's join: in q's memory, when the products are done
@@ -76,12 +78,12 @@ struct Smem {
 };
 using PrefixSmem1 = Smem<1, 0>;
 using PrefixSmem2 = Smem<2, 0>;
-using WindowSmem1 = Smem<1, 8>;
-using WindowSmem2 = Smem<2, 16>;
-static_assert(sizeof(PrefixSmem2) + 1024 <= 226 * 1024 && sizeof(WindowSmem2) + 1024 <= 226 * 1024,
-              "host requests 226 KB of dynamic shared memory (2 tiles)");
-static_assert(sizeof(PrefixSmem1) + 1024 <= 106 * 1024 && sizeof(WindowSmem1) + 1024 <= 106 * 1024,
-              "host requests 106 KB of dynamic shared memory (1 tile)");
+using WindowSmem1 = Smem<1, 64>;
+using WindowSmem2 = Smem<2, 256>;
+static_assert(sizeof(PrefixSmem2) + 1024 <= 227 * 1024 && sizeof(WindowSmem2) + 1024 <= 227 * 1024,
+              "host requests 227 KB of dynamic shared memory (2 tiles)");
+static_assert(sizeof(PrefixSmem1) + 1024 <= 108 * 1024 && sizeof(WindowSmem1) + 1024 <= 108 * 1024,
+              "host requests 108 KB of dynamic shared memory (1 tile)");
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
   float r;
@@ -153,15 +155,17 @@ __device__ __forceinline__ float2 load_remote2(uint32_t a) {
 }
 
 // The softmax threads hold a row of scores: with two tiles they take registers
-// that the other warps do not need (65,536 / 384 threads = 168 at launch;
-// 256 x 208 + 128 x 88 = 384 x 168).
-template <int QT>
+// that the other warps do not need. With epilogue warps 512 threads have 128
+// each at launch (256 x 200 + 256 x 56), without 384 have 168 (256 x 208 + 128 x 88).
+template <int QT, bool EPILOGUE>
 __device__ __forceinline__ void take_registers() {
-  if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  if constexpr (QT == 2 && EPILOGUE) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+  else if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
 }
-template <int QT>
+template <int QT, bool EPILOGUE>
 __device__ __forceinline__ void give_registers() {
-  if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if constexpr (QT == 2 && EPILOGUE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  else if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
 
 // What the body needs of a CTA's work: its items one after another (next() in
@@ -171,18 +175,21 @@ __device__ __forceinline__ void give_registers() {
 template <class Work, class Smem>
 __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log2) {
   constexpr int QT = Smem::QT, SLOTS = Smem::SLOTS;
+  constexpr bool EPILOGUE = Work::EPILOGUE;  // warps of their own normalise and store O
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&sm.q_full, 1);
-    mbar_init(&sm.q_empty, 1);
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&sm.kv_full[s], 1);
       mbar_init(&sm.kv_empty[s], 1);
     }
     for (int t = 0; t < QT; ++t) {
+      mbar_init(&sm.q_full[t], 1);
+      mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_full[t], 1);
       mbar_init(&sm.p_full[t], 4);
       mbar_init(&sm.o_full[t], 1);
+      mbar_init(&sm.l_full[t], 4);
+      mbar_init(&sm.o_empty[t], 4);
     }
     sm.abort = 0;
     fence_barrier_init();
@@ -202,7 +209,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
 
   if (warp == 4 * QT) {
     // ---------------- TMA producer ----------------
-    give_registers<QT>();
+    give_registers<QT, EPILOGUE>();
     if (lane == 0) {
       int slot = 0, items = 0;
       uint32_t phase = 0;
@@ -212,13 +219,11 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
 #pragma unroll 1
           for (int v = 0; v < 2; ++v) {
             // q comes behind the first K, whose slot is free before the last item's q is
-            if (i == 0 && v == 1) {
-              if (!mbar_wait(&sm.q_empty, (items & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
-                ok = false;
-                break;
-              }
-              w.load_q(sm, &sm.q_full);
+            for (int t = 0; i == 0 && v == 1 && t < QT; ++t) {
+              ok = ok && mbar_wait(&sm.q_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY);
+              if (ok) w.load_q(sm, &sm.q_full[t], t);
             }
+            if (!ok) break;
             if (!mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
               ok = false;
               break;
@@ -244,7 +249,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
     }
   } else if (warp == 4 * QT + 1) {
     // ---------------- MMA issuer ----------------
-    give_registers<QT>();
+    give_registers<QT, EPILOGUE>();
     // The warp stays together: what the instructions take (descriptors, addresses)
     // is then computed once for the warp, and one elected lane issues them.
     constexpr uint32_t id_qk = idesc_bf16<128, 128>(), id_qk_few = idesc_bf16<128, FEW>();
@@ -276,32 +281,43 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
       if (issuer) mma_commit(bar);
     };
     uint32_t tiles = 0, items = 0;  // key tiles and items so far
-    bool ok = true;
-    for (; ok && w.next(); ++items) {
-      const int n = w.n;
-      if (n == 0) continue;
-      ok = mbar_wait(&sm.q_full, items & 1, FB_KERR_TIMEOUT_FULL) &&
-           mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+    bool ok = true, more = w.next() && w.n > 0;
+    int n = w.n;
+    bool few = w.few;
+    if (more) {
+      ok = mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+      for (int t = 0; t < QT; ++t) ok = ok && mbar_wait(&sm.q_full[t], 0, FB_KERR_TIMEOUT_FULL);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      // S and P of the last item are done with: its last P V is issued, behind its last softmax
-      for (int t = 0; t < QT; ++t) qk(t, w.few ? id_qk_few : id_qk);
-      commit(&sm.kv_empty[kslot]);
-      if (n == 1) commit(&sm.q_empty);
-      next(kslot, kphase);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < QT; ++t) {
+          qk(t, few ? id_qk_few : id_qk);
+          if (n == 1) commit(&sm.q_empty[t]);
+        }
+        commit(&sm.kv_empty[kslot]);
+        next(kslot, kphase);
+      }
+    }
+    for (; ok && more; ++items) {
       for (int i = 0; ok && i < n; ++i, ++tiles) {
+        // Behind P_t V_i comes the next key tile's product for the same query
+        // tile: of the next item, behind the last of this one, so that neither
+        // query tile waits for the other one's end.
+        const bool last = i == n - 1;
+        if (last) more = w.next();
+        const bool next_qk = !last || more, next_ends = last ? w.n == 1 : i + 2 == n;
+        const uint32_t next_id = last && w.few ? id_qk_few : id_qk;
         ok = mbar_wait(&sm.kv_full[vslot], vphase, FB_KERR_TIMEOUT_FULL);
         const uint64_t vd = v_desc + vslot * (TILE / 16);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           ok = ok && mbar_wait(&sm.p_full[t], tiles & 1, FB_KERR_TIMEOUT_TMEM);
-          if (t == 0 && i + 1 < n) ok = ok && mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+          if (EPILOGUE && i == 0) ok = ok && mbar_wait(&sm.o_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_TMEM);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           if (issuer) {
-            const int steps = i == 0 && w.few ? FEW / 16 : 8;
+            const int steps = i == 0 && few ? FEW / 16 : 8;
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // K = 128 keys, 16 per MMA
               if (k < steps)
@@ -309,21 +325,30 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
                             (i > 0 || k > 0) ? 1u : 0u);
           }
           if (t == QT - 1) commit(&sm.kv_empty[vslot]);
-          if (i + 1 < n) qk(t, id_qk);
-          else commit(&sm.o_full[t]);
+          if (last) commit(&sm.o_full[t]);
+          if (next_qk) {
+            if (t == 0) ok = mbar_wait(&sm.kv_full[kslot], kphase, FB_KERR_TIMEOUT_FULL);
+            if (last) ok = ok && mbar_wait(&sm.q_full[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            qk(t, next_id);
+            if (next_ends) commit(&sm.q_empty[t]);
+          }
         }
-        if (ok && i + 1 < n) {
+        if (ok && next_qk) {
           commit(&sm.kv_empty[kslot]);
-          if (i + 2 == n) commit(&sm.q_empty);
           next(kslot, kphase);
         }
         next(vslot, vphase);
       }
+      n = w.n;
+      few = w.few;
     }
     if (!ok) sm.abort = 1;
   } else if (warp < 4 * QT) {
     // ---------------- softmax + epilogue ----------------
-    take_registers<QT>();
+    take_registers<QT, EPILOGUE>();
     const int t = warp >> 2;                         // query tile
     const int r = (warp & 3) * 32 + lane;            // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -453,21 +478,55 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
         }
         tmem_st_wait();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[t]);
         l_run = l_run * alpha + ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y));
         m_run = m_new;
+        if (EPILOGUE && i == n - 1) {
+          // Not before the epilogue has read the last item's: with one key tile per
+          // item nothing else would keep this warp from running two items ahead.
+          if (!mbar_wait(&sm.o_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_TMEM)) ok = false;
+          sm.l[t][r] = l_run;
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.p_full[t]);
+          if (EPILOGUE && i == n - 1) mbar_arrive(&sm.l_full[t]);
+        }
       }
-      for (int i = 0; ok && n > 0 && i < QT; ++i)  // of every tile: a store may reuse the ring
-        if (i == t || Work::REUSES_RING) ok = mbar_wait(&sm.o_full[i], items & 1, FB_KERR_TIMEOUT_TMEM);
-      if (ok) {
-        tc_fence_after();
-        w.store(sm, t, r, t_o, m_run, l_run);
+      if constexpr (!EPILOGUE) {
+        for (int i = 0; ok && n > 0 && i < QT; ++i)  // of every tile: a store may reuse the ring
+          if (i == t || Work::JOINS) ok = mbar_wait(&sm.o_full[i], items & 1, FB_KERR_TIMEOUT_TMEM);
+        if (ok) {
+          tc_fence_after();
+          w.store(sm, t, r, t_o, m_run, l_run, [] {});
+        }
       }
     }
     if (!ok) sm.abort = 1;
+  } else if (EPILOGUE && warp >= 4 * QT + 4) {
+    // ---------------- epilogue ----------------
+    // O of an item is read while the softmax warps are at the next one.
+    give_registers<QT, EPILOGUE>();
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t items = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (; ok && w.next(); ++items)
+#pragma unroll 1
+      for (int t = 0; ok && t < QT; ++t) {
+        ok = mbar_wait(&sm.l_full[t], items & 1, FB_KERR_TIMEOUT_TMEM) &&
+             mbar_wait(&sm.o_full[t], items & 1, FB_KERR_TIMEOUT_TMEM);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        w.store(sm, t, r, tmem + (QT + t) * 128 + lane_base, 0.f, sm.l[t][r], [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.o_empty[t]);
+        });
+      }
+    if (!ok) sm.abort = 1;
   } else {
-    give_registers<QT>();
+    give_registers<QT, EPILOGUE>();
   }
   w.finish(sm);
   tc_fence_before();
@@ -493,131 +552,114 @@ struct WindowWork {
   const CUtensorMap *tmQ, *tmK, *tmV;
   bf16* out;
   const int *cu_seqlens, *tile_seq, *tile_start;
-  int ld_o, n_tiles, heads, group, window, all_sinks;
-  // Items go tile by tile, head by head: one of `tile` and `head` is next. What
-  // its tables say is read two items ahead (the tile's prompt), then one (where
-  // that begins and ends), so that nothing waits for them.
-  int tile, head, step_tile, step_head;
-  int seq2, start2, s0_1, s1_1, start1, tile1, head1;
-  int head0, kvh, s0, s1, qp0, n, n_sink, first, sinks;
+  int ld_o, rows, n_seqs, n_tiles, heads, group, window, all_sinks;
+  // Items go tile by tile, head by head. What the tables say of an item is read
+  // two items ahead (the tile's prompt), then one (where that begins and ends), so
+  // that nothing waits for them.
+  int item;  // one ahead
+  int seq2, start2, s0_1, s1_1, start1;
+  int head0, s0, s1, qp0, n, n_sink, first, sinks;
   bool few;
 
-  __device__ __forceinline__ void advance() {
-    s0_1 = s1_1 = 0;
+  __device__ __forceinline__ void read_tile(int i) {
+    const int tile = min(i / heads, n_tiles - 1);
+    seq2 = tile_seq[tile];
+    start2 = tile_start[tile];
+  }
+  __device__ __forceinline__ void read_prompt() {
+    const int seq = min(max(seq2, 0), n_seqs - 1);  // whatever the tables say, nothing outside the tensors is touched
     start1 = start2;
-    tile1 = tile;
-    head1 = head;
-    if (tile1 < n_tiles) {
-      s0_1 = cu_seqlens[seq2];
-      s1_1 = cu_seqlens[seq2 + 1];
-    }
-    tile += step_tile;
-    head += step_head;
-    if (head >= heads) {
-      head -= heads;
-      ++tile;
-    }
-    if (tile < n_tiles) {
-      seq2 = tile_seq[tile];
-      start2 = tile_start[tile];
-    }
+    s0_1 = cu_seqlens[seq];
+    s1_1 = cu_seqlens[seq + 1];
   }
   __device__ __forceinline__ void start() {
-    tile = blockIdx.x / heads;
-    head = blockIdx.x % heads;
-    step_tile = gridDim.x / heads;
-    step_head = gridDim.x % heads;
-    if (tile < n_tiles) {
-      seq2 = tile_seq[tile];
-      start2 = tile_start[tile];
-    }
-    advance();
+    item = blockIdx.x;
+    read_tile(item);
+    read_prompt();
+    read_tile(item + gridDim.x);
   }
   __device__ __forceinline__ bool next() {
-    for (; tile1 < n_tiles; advance()) {
-      s0 = s0_1;
-      s1 = s1_1;
+    for (bool found = false; !found;) {
+      if (item >= n_tiles * heads) return false;
+      s0 = max(s0_1, 0);
+      s1 = min(s1_1, rows);
       qp0 = start1;
-      const int end = min(qp0 + BQ, s1 - s0);  // queries and keys of this tile end here
-      if (qp0 < 0 || qp0 >= end) continue;     // a tile table that does not match cu_seqlens
-      head0 = head1 * QT;
-      kvh = head0 / group;
-      const int last = (end - 1) / BK, in_window = max(qp0 - window + 1, 0) / BK;
-      sinks = min(all_sinks, end);
-      n_sink = min((sinks + BK - 1) / BK, last + 1);
-      first = max(in_window, n_sink);
-      n = n_sink + last + 1 - first;
-      few = n_sink == 1 && sinks <= FEW && in_window > 0;
-      advance();
-      return true;
+      head0 = item % heads * QT;
+      item += gridDim.x;
+      read_prompt();
+      read_tile(item + gridDim.x);
+      found = qp0 >= 0 && qp0 < s1 - s0;  // (else: a tile table that does not match cu_seqlens)
     }
-    return false;
+    const int end = min(qp0 + BQ, s1 - s0);  // queries and keys of this tile end here
+    const int last = (end - 1) / BK, in_window = max(qp0 - window + 1, 0) / BK;
+    sinks = min(all_sinks, end);
+    n_sink = min((sinks + BK - 1) / BK, last + 1);
+    first = max(in_window, n_sink);
+    n = n_sink + last + 1 - first;
+    few = n_sink == 1 && sinks <= FEW && in_window > 0;
+    return true;
   }
   __device__ __forceinline__ int key0(int i) const { return (i < n_sink ? i : i - n_sink + first) * BK; }
   __device__ __forceinline__ bool zero_row(int i, int r) const { return key0(i) + r >= s1 - s0; }
   __device__ __forceinline__ void clear_q(Smem&) const {}
-  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar) const {
-    mbar_arrive_expect_tx(bar, QT * TILE);
-    for (int t = 0; t < QT; ++t)
-      for (int h = 0; h < 2; ++h) tma_load_2d(sm.q[t] + h * HALF, tmQ, bar, (head0 + t) * D + h * 64, s0 + qp0);
+  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar, int t) const {
+    mbar_arrive_expect_tx(bar, TILE);
+    for (int h = 0; h < 2; ++h) tma_load_2d(sm.q[t] + h * HALF, tmQ, bar, (head0 + t) * D + h * 64, s0 + qp0);
   }
   __device__ __forceinline__ void load_kv(uint8_t* dst, uint64_t* bar, int i, int v) const {
     const int row = s0 + key0(i);
-    for (int h = 0; h < 2; ++h) tma_load_2d(dst + h * HALF, v ? tmV : tmK, bar, kvh * D + h * 64, row);
+    for (int h = 0; h < 2; ++h) tma_load_2d(dst + h * HALF, v ? tmV : tmK, bar, head0 / group * D + h * 64, row);
   }
   __device__ __forceinline__ void row_range(int, int r, int& hi, int& lo) const {
     const int qpos = qp0 + r;
     hi = s0 + qpos < s1 ? qpos : -1;
     lo = qpos - window + 1;
   }
-  static constexpr bool REUSES_RING = false;
   __device__ __forceinline__ void finish(Smem&) const {}
-  // Rows go through shared memory, 16-byte chunks swizzled by the row, so that a
-  // store instruction writes two whole rows of the head: straight from a row per
-  // thread it would touch 32 lines, and the stores of a tile took as long as two
-  // key tiles.
-  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float, float l) const {
+  static constexpr bool EPILOGUE = QT == 2, JOINS = false;
+  // Rows go through shared memory (32 dims of them at a time, or whole), 16-byte
+  // chunks swizzled by the row, so that a store instruction writes 64 bytes of
+  // eight rows or two whole rows: straight from a row per thread it would touch 32
+  // lines, and the stores of a tile took as long as two key tiles. `read` is called
+  // when O has been read: with whole rows, before any of them is stored.
+  template <class Read>
+  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float, float l, Read read) const {
+    constexpr int CHUNKS = Smem::STAGE / 16, ROWS = 32 / CHUNKS;  // chunks of a staged row; rows of a store
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int lane = r & 31, row0 = s0 + qp0 + (r & ~31);
-    uint4 packed[16];
-#pragma unroll
+    const int lane = r & 31, row0 = s0 + qp0 + (r & ~31), my_row = lane / CHUNKS, my_chunk = lane % CHUNKS;
+    uint8_t* stage = sm.stage[r >> 5];
+    auto at = [&](int row, int chunk) {
+      const int swizzle = CHUNKS == 16 ? row & 15 : (row >> 1) & 3;
+      return reinterpret_cast<uint4*>(stage + row * Smem::STAGE + ((chunk ^ swizzle) << 4));
+    };
+#pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
       tmem_ld32(t_o + c, o);
       tmem_ld_wait();
+      if (c == D - 32) read();
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
+      for (int e = 0; e < 4; ++e) {
         float f[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[e + x]) * inv;
-        packed[(c + e) / 8] = pack8(f);
+        for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * inv;
+        *at(lane, CHUNKS == 16 ? c / 8 + e : e) = pack8(f);
       }
-    }
-    uint8_t* stage = sm.stage[t * 4 + (r >> 5)];
-#pragma unroll 1
-    for (int p = 0; p < 32; p += Smem::ROWS) {
+      if (CHUNKS == 16 && c < D - 32) continue;
       __syncwarp();
-      if (lane >= p && lane < p + Smem::ROWS) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          *reinterpret_cast<uint4*>(stage + (lane - p) * 256 + ((e ^ (lane & 15)) << 4)) = packed[e];
-      }
+      bf16* to = out + static_cast<size_t>(row0 + my_row) * ld_o + (head0 + t) * D + (CHUNKS == 16 ? 0 : c) + my_chunk * 8;
+#pragma unroll 4
+      for (int row = my_row; row < 32; row += ROWS, to += static_cast<size_t>(ROWS) * ld_o)
+        if (row0 + row < s1) *reinterpret_cast<uint4*>(to) = *at(row, my_chunk);
       __syncwarp();
-#pragma unroll
-      for (int e = 0; e < Smem::ROWS / 2; ++e) {
-        const int row = 2 * e + (lane >> 4), chunk = lane & 15;
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 256 + ((chunk ^ ((row + p) & 15)) << 4));
-        if (row0 + p + row < s1)
-          *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + p + row) * ld_o + (head0 + t) * D + chunk * 8) = v;
-      }
     }
   }
 };
 
 template <class Smem>
 __device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUtensorMap* tmK, const CUtensorMap* tmV,
-                                               bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,
-                                               const int* tile_start, int n_tiles, int Hq, int Hkv, int window,
+                                               bf16* out, int ld_o, int rows, int n_seqs, const int* cu_seqlens,
+                                               const int* tile_seq, const int* tile_start, int n_tiles, int Hq, int Hkv, int window,
                                                int sinks, float scale_log2) {
   pdl_wait();
   WindowWork<Smem> w;
@@ -626,6 +668,8 @@ __device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUt
   w.tmV = tmV;
   w.out = out;
   w.ld_o = ld_o;
+  w.rows = rows;
+  w.n_seqs = n_seqs;
   w.cu_seqlens = cu_seqlens;
   w.tile_seq = tile_seq;
   w.tile_start = tile_start;
@@ -682,12 +726,11 @@ struct PrefixWork {
           make_uint4(0, 0, 0, 0);
     }
   }
-  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar) const {
-    mbar_arrive_expect_tx(bar, QT * 2 * G * nb * 128);
-    for (int t = 0; t < QT; ++t)
-      for (int g = 0; g < G; ++g)
-        for (int h = 0; h < 2; ++h)
-          tma_load_2d(sm.q[t] + h * HALF + g * nb * 128, tmQ, bar, (kvh * G + g) * D + h * 64, it.row0 + t * nb);
+  __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar, int t) const {
+    mbar_arrive_expect_tx(bar, 2 * G * nb * 128);
+    for (int g = 0; g < G; ++g)
+      for (int h = 0; h < 2; ++h)
+        tma_load_2d(sm.q[t] + h * HALF + g * nb * 128, tmQ, bar, (kvh * G + g) * D + h * 64, it.row0 + t * nb);
   }
   __device__ __forceinline__ void load_kv(uint8_t* dst, uint64_t* bar, int i, int v) const {
 #pragma unroll
@@ -715,12 +758,13 @@ struct PrefixWork {
     const int b = row_of(t, r);
     return r < G * nb && b < it.rows ? (it.row0 + b) * static_cast<long long>(Hq) + kvh * G + r / nb : -1;
   }
-  static constexpr bool REUSES_RING = true;
+  static constexpr bool EPILOGUE = false, JOINS = true;
   // O rows of the tiles in the ring's memory, 16-byte chunks swizzled by the row.
   __device__ __forceinline__ static uint32_t o_at(Smem& sm, int t, int r, int chunk) {
     return smem_u32(sm.kv[0]) + (t * BQ + r) * (D * 4) + ((chunk ^ (r & 31)) << 4);
   }
-  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float m, float l) const {
+  template <class Read>
+  __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float m, float l, Read) const {
     sm.ml(t)[r] = make_float2(m, l);
     if (n == 0) return;  // O is nothing
 #pragma unroll 1
@@ -818,11 +862,12 @@ struct TileMaps {
 // q [T, Hq * 128], k, v [T, Hkv * 128]: maps over the packed rows, boxes of 128
 // rows. n_tiles query tiles of tile_seq / tile_start. out [T, ld_o] bf16, head h at columns h * 128; rows outside every prompt are not written.
 #define FB_WINDOW_PREFILL(QT, CTAS)                                                                               \
-  extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_window_prefill_q##QT(                      \
-      const __grid_constant__ TileMaps maps, bf16* out, int ld_o, const int* cu_seqlens, const int* tile_seq,     \
-      const int* tile_start, int n_tiles, int Hq, int Hkv, int window, int sinks, float scale_log2) {             \
-    window_prefill<WindowSmem##QT>(&maps.q, &maps.k, &maps.v, out, ld_o, cu_seqlens, tile_seq, tile_start, n_tiles, Hq, Hkv,  \
-                       window, sinks, scale_log2);                                                                        \
+  extern "C" __global__ void __launch_bounds__(QT == 2 ? 512 : 192, CTAS) fb_window_prefill_q##QT(                \
+      const __grid_constant__ TileMaps maps, bf16* out, int ld_o, int rows, int n_seqs, const int* cu_seqlens,    \
+      const int* tile_seq, const int* tile_start, int n_tiles, int Hq, int Hkv, int window, int sinks,            \
+      float scale_log2) {                                                                                         \
+    window_prefill<WindowSmem##QT>(&maps.q, &maps.k, &maps.v, out, ld_o, rows, n_seqs, cu_seqlens, tile_seq,      \
+                                   tile_start, n_tiles, Hq, Hkv, window, sinks, scale_log2);                      \
   }
 FB_WINDOW_PREFILL(1, 2)
 FB_WINDOW_PREFILL(2, 1)

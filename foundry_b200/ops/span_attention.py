@@ -24,8 +24,9 @@ from .attention import LOG2E, PAGE
 _SPAN, _TILE = "attention_span", "attention_tile"
 MAX_GROUP = 16
 SPAN_SMEM = 74 * 1024
-TILE_SMEM = {1: 106 * 1024, 2: 226 * 1024}
-TILE_THREADS = {1: 192, 2: 384}
+TILE_SMEM = {1: 108 * 1024, 2: 227 * 1024}
+PREFIX_THREADS = {1: 192, 2: 384}  # by query tiles per CTA
+PREFILL_THREADS = {1: 192, 2: 512}
 TILE = 128  # queries (and keys) of a tile
 MAX_CLUSTER = 8  # CTAs that share a prefix's pages between them
 _BF16, _I32 = torch.bfloat16, torch.int32
@@ -264,7 +265,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         maps = core().make_tmaps_bf16([
             (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0),
             (k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0), (v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0)])
-        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (TILE_THREADS[plan.tiles],), [
+        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (PREFIX_THREADS[plan.tiles],), [
             maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
             ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, blocks, scale * LOG2E],
             TILE_SMEM[plan.tiles], _rt.raw_stream(), (plan.splits,))
@@ -298,15 +299,17 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     for x in (cu_seqlens, tile_seq, tile_start):
         if not (x.dtype is _I32 and x.dim() == 1 and x.is_contiguous()):
             raise ValueError("cu_seqlens and the tile tables must be contiguous int32")
-    n_tiles = tile_seq.shape[0]
-    if tile_start.shape[0] != n_tiles or cu_seqlens.shape[0] < 1:
+    n_tiles, n_seqs = tile_seq.shape[0], cu_seqlens.shape[0] - 1
+    if tile_start.shape[0] != n_tiles or n_seqs < 0:
         raise ValueError("tile tables of different lengths, or no cu_seqlens")
+    if n_tiles * n_q >= 1 << 30:
+        raise ValueError(f"{n_tiles} tiles of {n_q} heads are too many")
     _check_device(q, k, v, out, cu_seqlens, tile_seq, tile_start)
-    if not n_tiles or not t:
+    if not n_tiles or not n_seqs or not t:
         return out
     qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
     _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (min(n_tiles * (n_q // qt), _rt.sm_count() * (3 - qt)),),
-               (TILE_THREADS[qt],), [
-        core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), cu_seqlens.data_ptr(), tile_seq.data_ptr(),
-        tile_start.data_ptr(), n_tiles, n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
+               (PREFILL_THREADS[qt],), [
+        core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), t, n_seqs, cu_seqlens.data_ptr(),
+        tile_seq.data_ptr(), tile_start.data_ptr(), n_tiles, n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
     return out

@@ -230,6 +230,8 @@ def test_prefix_decode_agrees_with_decode_attention_in_a_captured_graph():
 @pytest.mark.parametrize("lens,window,sinks", [
     ([1], 1, 0), ([1, 2, 0, 127, 128, 129], 64, 4), ([300, 5, 700], 128, 1), ([513], 1000, 4), ([900, 130], 200, 130),
     ([1100], 1, 300), ([640], 257, 0),
+    # many items for every CTA, of one key tile, of few, of both in turn
+    ([(37 * i) % 128 + 1 for i in range(250)], 64, 4), ([(531 * i) % 900 for i in range(40)], 128, 4),
 ])
 def test_window_prefill(n_q, n_kv, lens, window, sinks):
     """Packed prompts as slices of one matrix, NaN behind the last one."""
@@ -248,6 +250,7 @@ def test_window_prefill(n_q, n_kv, lens, window, sinks):
     ts, tst = ops.prefill_tiles(lens)
     ops.window_prefill_attention(q, k, v, out, _i32(cu), _i32(ts), _i32(tst), n_q, n_kv, window, sinks)
     assert (out[t:] == 7).all()
+    assert ops.status("attention_tile") == 0
     for a, b in zip(cu, cu[1:]):
         if a == b:
             continue
