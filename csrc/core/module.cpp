@@ -8,7 +8,6 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
-#include <array>
 #include <chrono>
 #include <fstream>
 #include <mutex>
@@ -197,26 +196,94 @@ py::bytes rt_make_tmap_3d(uint64_t ptr, int dtype, uint64_t d0, uint64_t d1, uin
   return py::bytes(reinterpret_cast<const char*>(&m), sizeof(m));
 }
 
-// bf16 tensor maps with 64-column x box_rows boxes and the 128-byte swizzle, one
-// after another in one byte string (a kernel that needs several takes them as
-// one struct): (address, columns, rows, row stride in bytes, box rows, planes,
-// plane stride in bytes) each; planes = 0 for two dimensions.
-py::bytes rt_make_tmaps_bf16(const std::vector<std::array<uint64_t, 7>>& maps) {
-  std::vector<CUtensorMap> m(maps.size());
-  for (size_t i = 0; i < maps.size(); ++i) {
-    const auto& a = maps[i];
+// launch() for the ops whose calls are short: everything comes as plain numbers
+// in one tuple, without a conversion to a container on the way.
+//
+//   fn, grid x, grid y, block x, shared memory, stream, cluster x, pdl,
+//   number of tensor maps, 7 numbers for each of them, kernel arguments
+//
+// The maps (bf16, boxes of 64 columns x box_rows, 128-byte swizzle) fill the
+// kernel's first parameter, a struct of them: (address, columns, rows, row stride
+// in bytes, box rows, planes, plane stride in bytes), planes = 0 for two dimensions.
+void rt_launch_mapped(py::args all) {
+  const Py_ssize_t count = PyTuple_GET_SIZE(all.ptr());
+  Py_ssize_t at = 0;
+  auto next = [&]() -> uint64_t {
+    if (at >= count) throw std::runtime_error("launch_mapped: too few numbers");
+    const uint64_t v = PyLong_AsUnsignedLongLongMask(PyTuple_GET_ITEM(all.ptr(), at++));
+    if (v == static_cast<uint64_t>(-1) && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+  };
+  CUfunction f = reinterpret_cast<CUfunction>(next());
+  const FuncInfo& info = func_info(f);
+  CUlaunchConfig cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDimX = static_cast<unsigned>(next());
+  cfg.gridDimY = static_cast<unsigned>(next());
+  cfg.blockDimX = static_cast<unsigned>(next());
+  cfg.gridDimZ = cfg.blockDimY = cfg.blockDimZ = 1;
+  cfg.sharedMemBytes = static_cast<unsigned>(next());
+  cfg.hStream = reinterpret_cast<CUstream>(next());
+  CUlaunchAttribute attrs[2];
+  memset(attrs, 0, sizeof(attrs));
+  unsigned n = 0;
+  if (const unsigned cluster = static_cast<unsigned>(next()); cluster > 1) {
+    attrs[n].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+    attrs[n].value.clusterDim.x = cluster;
+    attrs[n].value.clusterDim.y = attrs[n].value.clusterDim.z = 1;
+    ++n;
+  }
+  if (next()) {
+    attrs[n].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+    attrs[n].value.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = n ? attrs : nullptr;
+  cfg.numAttrs = n;
+  constexpr size_t MAX_PARAMS = 40, MAX_MAPS = 8;
+  alignas(64) CUtensorMap maps[MAX_MAPS];
+  uint64_t values[MAX_PARAMS];
+  void* ptrs[MAX_PARAMS];
+  const size_t n_maps = next();
+  if (n_maps > MAX_MAPS || info.params.size() > MAX_PARAMS)
+    throw std::runtime_error("launch_mapped: too many tensor maps or parameters");
+  for (size_t i = 0; i < n_maps; ++i) {
+    uint64_t a[7];
+    for (uint64_t& v : a) v = next();
     cuuint64_t dims[3] = {a[1], a[2], a[5]};
     cuuint64_t strides[2] = {a[3], a[6]};
     cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a[4]), 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    check_drv(fb_driver()->cuTensorMapEncodeTiled(&m[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a[5] ? 3 : 2,
+    check_drv(fb_driver()->cuTensorMapEncodeTiled(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a[5] ? 3 : 2,
                                                   reinterpret_cast<void*>(a[0]), dims, strides, box, estr,
                                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
               "cuTensorMapEncodeTiled");
   }
-  return py::bytes(reinterpret_cast<const char*>(m.data()), m.size() * sizeof(CUtensorMap));
+  const size_t first = n_maps ? 1 : 0;
+  if (n_maps && (info.params.empty() || info.params[0].second != n_maps * sizeof(CUtensorMap)))
+    throw std::runtime_error("launch_mapped: the kernel's first parameter is not a struct of " +
+                             std::to_string(n_maps) + " tensor maps");
+  if (static_cast<size_t>(count - at) != info.params.size() - first)
+    throw std::runtime_error("kernel expects " + std::to_string(info.params.size() - first) + " arguments, got " +
+                             std::to_string(count - at));
+  if (n_maps) ptrs[0] = maps;
+  for (size_t i = first; i < info.params.size(); ++i) {
+    PyObject* o = PyTuple_GET_ITEM(all.ptr(), at);
+    if (info.params[i].second > 8)
+      throw std::runtime_error("launch_mapped: parameter " + std::to_string(i) + " is no number");
+    if (PyFloat_Check(o)) {
+      const float v = static_cast<float>(PyFloat_AS_DOUBLE(o));
+      values[i] = 0;
+      memcpy(&values[i], &v, sizeof(v));
+      ++at;
+    } else {
+      values[i] = next();
+    }
+    ptrs[i] = &values[i];
+  }
+  check_drv(fb_driver()->cuLaunchKernelEx(&cfg, f, ptrs, nullptr), "cuLaunchKernelEx");
 }
 
 // Address of a __device__ global of an image (e.g. an error-status word).
@@ -441,7 +508,7 @@ PYBIND11_MODULE(_C, m) {
         py::arg("row_stride_bytes"), py::arg("box_inner"), py::arg("box_outer"), py::arg("swizzle"),
         py::arg("l2promo") = 2);
   m.def("make_tmap_3d", &rt_make_tmap_3d);
-  m.def("make_tmaps_bf16", &rt_make_tmaps_bf16);
+  m.def("launch_mapped", &rt_launch_mapped);
   m.def("get_global", &rt_get_global);
   m.def("func_attr", &rt_func_attr);
   m.def("func_num_params", [](uintptr_t fn) { return func_info(reinterpret_cast<CUfunction>(fn)).params.size(); });

@@ -85,20 +85,27 @@ def pdl_active() -> bool:
 
 
 def launch(image: str, name: str, grid, block, args, smem: int = 0, stream: int | None = None,
-           cluster=(), after_own: bool = False) -> None:
-    """``after_own``: the launch right before it on this stream is one of the
-    same op; this kernel may be set up while that one runs (it waits for it
-    before it reads anything, as every kernel of ``PDL_IMAGES`` does)."""
+           cluster=()) -> None:
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
     fn = function(image, name, smem)
     core().launch(fn, tuple(grid), tuple(block), smem, stream, args, tuple(cluster),
-                  (after_own and PDL_ENABLED) or (pdl_active() and image in PDL_IMAGES))
+                  pdl_active() and image in PDL_IMAGES)
 
 
-def raw_stream() -> int:
-    """The current stream's handle, without the Stream object around it."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+def launch_mapped(image: str, name: str, grid_x: int, grid_y: int, threads: int, smem: int, n_maps: int, *numbers,
+                  cluster: int = 1, after_own: bool = False) -> None:
+    """``launch`` on the current stream for ops whose calls are short: numbers
+    only, ``n_maps`` times 7 of them for the tensor maps that the kernel takes
+    as its first parameter (csrc/core/module.cpp), then its arguments.
+
+    ``after_own``: the launch right before it on this stream is one of the
+    same op; this kernel may be set up while that one runs (it waits for it
+    before it reads anything, as every kernel of ``PDL_IMAGES`` does)."""
+    fn = _funcs.get((image, name, smem)) or function(image, name, smem)
+    core().launch_mapped(fn, grid_x, grid_y, threads, smem,
+                         torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()), cluster,
+                         PDL_ENABLED and (after_own or getattr(_pdl, "depth", 0) > 0), n_maps, *numbers)
 
 
 def status(image: str) -> int:

@@ -33,6 +33,7 @@ class LogprobWorkspace:
         self.sums = empty((2 * self.ctas * 4,), torch.float32)
         self.keys = empty((2 * self.ctas * MAX_TOP,), torch.int64)
         self.tickets = zeros((self.ctas,), torch.int32)
+        self.sums_ptr, self.keys_ptr, self.tickets_ptr = self.sums.data_ptr(), self.keys.data_ptr(), self.tickets.data_ptr()
 
     def clear(self) -> None:
         self.tickets.zero_()
@@ -91,6 +92,6 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
     if not t:
         return
     share, pitch = share_of(t, v, ws.ctas)
-    _rt.launch(_IMG, _NAMES[logits.dtype], (min(ws.ctas, math.ceil(t * pitch / share)),), (256,), [
-        logits.data_ptr(), logits.stride(0), *ptrs, ws.sums.data_ptr(), ws.keys.data_ptr(), ws.tickets.data_ptr(),
-        share, pitch, t, v, k], SMEM, _rt.raw_stream())
+    _rt.launch_mapped(
+        _IMG, _NAMES[logits.dtype], min(ws.ctas, math.ceil(t * pitch / share)), 1, 256, SMEM, 0, logits.data_ptr(),
+        logits.stride(0), *ptrs, ws.sums_ptr, ws.keys_ptr, ws.tickets_ptr, share, pitch, t, v, k)

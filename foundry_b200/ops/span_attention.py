@@ -17,7 +17,6 @@ import math
 
 import torch
 
-from .._native import core
 from . import _rt
 from .attention import LOG2E, PAGE
 
@@ -138,6 +137,8 @@ class SpanWorkspace:
         self.partials = partials
         self.prefix_o = empty((max(partials, 1) * 128,), torch.float32)
         self.prefix_ml = empty((max(partials, 1) * 2,), torch.float32)
+        self.o_ptr, self.ml_ptr, self.tickets_ptr = self.o.data_ptr(), self.ml.data_ptr(), self.tickets.data_ptr()
+        self.prefix_o_ptr, self.prefix_ml_ptr = self.prefix_o.data_ptr(), self.prefix_ml.data_ptr()
 
     def clear(self) -> None:
         self.tickets.zero_()
@@ -147,19 +148,19 @@ def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, d
           scale: float, plan: "PrefixPlan | None" = None) -> None:
     b, n_q, n_kv, blocks, max_blocks = dims
     g = n_q // n_kv
-    k, v, rows = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE
-    ld = q.stride(0) if b > 1 else n_q * 128
+    k, v, rows, q_ptr = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE, q.data_ptr()
     if ws.tickets.get_device() != q.get_device():
         raise ValueError("the workspace is on another device")
-    # q last: its heads are a dimension of their own (one box: a KV head's heads of one row)
-    maps = core().make_tmaps_bf16([(k, 128, rows, 256, PAGE, 0, 0), (v, 128, rows, 256, PAGE, 0, 0),
-                                   (k, 128, rows, 256, 16, 0, 0), (v, 128, rows, 256, 16, 0, 0),
-                                   (q.data_ptr(), 128, n_q, 256, g, b, ld * 2)])
-    _rt.launch(_SPAN, "fb_span_attn_g4" if g <= 4 else "fb_span_attn_g8" if g <= 8 else "fb_span_attn_g16",
-               (min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)),), (192,), [
-        maps, block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv,
-        g, window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(),
-        ws.o.data_ptr(), ws.ml.data_ptr(), ws.tickets.data_ptr(), scale * LOG2E], SPAN_SMEM, _rt.raw_stream(), (), plan is not None)
+    _rt.launch_mapped(
+        _SPAN, "fb_span_attn_g4" if g <= 4 else "fb_span_attn_g8" if g <= 8 else "fb_span_attn_g16",
+        min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)), 1, 192, SPAN_SMEM, 5,
+        k, 128, rows, 256, PAGE, 0, 0, v, 128, rows, 256, PAGE, 0, 0, k, 128, rows, 256, 16, 0, 0,
+        v, 128, rows, 256, 16, 0, 0,
+        # q's heads are a dimension of their own: one box holds a KV head's heads of one row
+        q_ptr, 128, n_q, 256, g, b, (q.stride(0) if b > 1 else n_q * 128) * 2,
+        block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv, g,
+        window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o_ptr, ws.prefix_ml_ptr, ws.o_ptr,
+        ws.ml_ptr, ws.tickets_ptr, scale * LOG2E, after_own=plan is not None)
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -216,6 +217,7 @@ class PrefixPlan:
         shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n and p]
         # two query tiles per CTA as soon as a group has more rows than one
         self.tiles = 2 if any(n > nb for n, _ in shared) else 1
+        self.kernel = f"fb_prefix_attn_q{self.tiles}"
         step = nb * self.tiles
         slots = max(1, _rt.sm_count() * (1 if self.tiles == 2 else 2) // n_kv)
         clusters = sum(math.ceil(n / step) for n, _ in shared)
@@ -262,13 +264,12 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError("the plan or the workspace is on another device")
     if plan.items_n:
         g, rows = n_q // n_kv, blocks * n_kv * PAGE
-        maps = core().make_tmaps_bf16([
-            (q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0),
-            (k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0), (v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0)])
-        _rt.launch(_TILE, f"fb_prefix_attn_q{plan.tiles}", (plan.items_n, n_kv), (PREFIX_THREADS[plan.tiles],), [
-            maps, plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(),
-            ws.prefix_o.data_ptr(), ws.prefix_ml.data_ptr(), g, n_q, n_kv, blocks, scale * LOG2E],
-            TILE_SMEM[plan.tiles], _rt.raw_stream(), (plan.splits,))
+        _rt.launch_mapped(
+            _TILE, plan.kernel, plan.items_n, n_kv, PREFIX_THREADS[plan.tiles], TILE_SMEM[plan.tiles], 3,
+            q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0,
+            k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0, v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0,
+            plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), ws.prefix_o_ptr,
+            ws.prefix_ml_ptr, g, n_q, n_kv, blocks, scale * LOG2E, cluster=plan.splits)
     _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan if plan.items_n else None)
     return out
 
@@ -295,7 +296,7 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
             ld = heads * 128
         if inner != 1 or ld % 8 or ld < heads * 128 or x.data_ptr() % 16:
             raise ValueError("q, k, v and out must be row-contiguous with 16-byte aligned rows that do not overlap")
-        maps.append((x.data_ptr(), heads * 128, t, ld * 2, TILE, 0, 0))
+        maps += x.data_ptr(), heads * 128, t, ld * 2, TILE, 0, 0
     for x in (cu_seqlens, tile_seq, tile_start):
         if not (x.dtype is _I32 and x.dim() == 1 and x.is_contiguous()):
             raise ValueError("cu_seqlens and the tile tables must be contiguous int32")
@@ -308,8 +309,9 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     if not n_tiles or not n_seqs or not t:
         return out
     qt = 2 if group % 2 == 0 else 1  # two heads of one KV head share its K/V tiles
-    _rt.launch(_TILE, f"fb_window_prefill_q{qt}", (min(n_tiles * (n_q // qt), _rt.sm_count() * (3 - qt)),),
-               (PREFILL_THREADS[qt],), [
-        core().make_tmaps_bf16(maps[:3]), out.data_ptr(), out.stride(0), t, n_seqs, cu_seqlens.data_ptr(),
-        tile_seq.data_ptr(), tile_start.data_ptr(), n_tiles, n_q, n_kv, window, sinks, scale * LOG2E], TILE_SMEM[qt], _rt.raw_stream())
+    _rt.launch_mapped(
+        _TILE, "fb_window_prefill_q2" if qt == 2 else "fb_window_prefill_q1",
+        min(n_tiles * (n_q // qt), _rt.sm_count() * (3 - qt)), 1, PREFILL_THREADS[qt], TILE_SMEM[qt], 3, *maps[:21],
+        out.data_ptr(), out.stride(0), t, n_seqs, cu_seqlens.data_ptr(), tile_seq.data_ptr(), tile_start.data_ptr(),
+        n_tiles, n_q, n_kv, window, sinks, scale * LOG2E)
     return out
