@@ -61,7 +61,8 @@ struct Smem {
   float red[4][NH];    // per-warp max, then per-warp sum, of every head
   float mrun[2][NH];   // running max per head: one in use, one for the next move
   int scan[THREADS / 32];
-  int total, first_row, first_off;
+  int first_row, first_off;
+  int2 first_length;
   uint32_t tmem;
   int last;
   int abort;
@@ -146,7 +147,7 @@ struct Walk {
   int2 ahead;  // the next row's length, read a row ahead: off the critical path
   __device__ __forceinline__ Walk(const Params& a, const Smem& sm, int begin, int e) : b(sm.first_row), at(begin), end(e) {
     if (begin >= end) return;
-    s = row_span(a, row_length(a, b));
+    s = row_span(a, sm.first_length);
     ahead = row_length(a, b + 1);
     kvh = sm.first_off / s.chunks;
     c0 = sm.first_off % s.chunks;
@@ -172,44 +173,42 @@ __device__ __forceinline__ int add_acq_rel(int* p, int v) {
   return old;
 }
 
-// Joins n partial results (max, sum) = *ml(k, h), output *part(k, h) into (m, l,
-// o) of two heads h = 0, 1. The loads of JOIN parts of both are on their way at a
-// time: one by one, their latency is what the join would take.
-constexpr int JOIN = 4;
+// One head's output row from the partial results of n pieces: *ml(k) = (max, sum),
+// part(k)[0 .. 127], a lane with four dims. The loads of JOIN pieces are on their
+// way at a time: one by one, their latency is what the join would take.
+constexpr int JOIN = 8;
 template <class Ml, class Part>
-__device__ __forceinline__ void join_parts(float (&m)[2], float (&l)[2], float (&o)[2], int n, Ml ml, Part part) {
+__device__ __forceinline__ float4 join_pieces(int n, Ml ml, Part part) {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
   for (int k0 = 0; k0 < n; k0 += JOIN) {
-    float2 s[JOIN][2];
-    float v[JOIN][2];
+    float2 s[JOIN];
+    float4 v[JOIN];
 #pragma unroll
-    for (int k = 0; k < JOIN; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[k][h] = __ldcg(ml(min(k0 + k, n - 1), h));  // without a branch, so that none waits for another
-        v[k][h] = __ldcg(part(min(k0 + k, n - 1), h));
-      }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float mx = m[h];
-#pragma unroll
-      for (int k = 1; k < JOIN; ++k)
-        if (k0 + k >= n) s[k][h] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int k = 0; k < JOIN; ++k) mx = fmaxf(mx, s[k][h].x);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      const float w = exp2f(m[h] - ref);
-      l[h] *= w;
-      o[h] *= w;
-#pragma unroll
-      for (int k = 0; k < JOIN; ++k) {
-        const float e = exp2f(s[k][h].x - ref);
-        l[h] = fmaf(s[k][h].y, e, l[h]);
-        o[h] = e > 0.f ? fmaf(v[k][h], e, o[h]) : o[h];
-      }
-      m[h] = mx;
+    for (int k = 0; k < JOIN; ++k) {
+      s[k] = __ldcg(ml(min(k0 + k, n - 1)));
+      v[k] = __ldcg(reinterpret_cast<const float4*>(part(min(k0 + k, n - 1))) + (threadIdx.x & 31));
     }
+    float mx = m;
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k) {
+      if (k0 + k >= n) s[k] = make_float2(-INFINITY, 0.f);
+      mx = fmaxf(mx, s[k].x);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx, w = exp2f(m - ref);
+    l *= w;
+    o = make_float4(o.x * w, o.y * w, o.z * w, o.w * w);
+#pragma unroll
+    for (int k = 0; k < JOIN; ++k) {
+      const float e = exp2f(s[k].x - ref);
+      l = fmaf(s[k].y, e, l);
+      o = make_float4(fmaf(v[k].x, e, o.x), fmaf(v[k].y, e, o.y), fmaf(v[k].z, e, o.z), fmaf(v[k].w, e, o.w));
+    }
+    m = mx;
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 template <int GP>
@@ -281,7 +280,8 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
   if (begin < end && begin >= before && begin < before + mine) {
     int off = begin - before, b = row0;
     for (;; ++b) {
-      const int len = row_span(a, row_length(a, b)).chunks * a.Hkv;
+      sm.first_length = row_length(a, b);
+      const int len = row_span(a, sm.first_length).chunks * a.Hkv;
       if (off < len) break;
       off -= len;
     }
@@ -512,8 +512,14 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
       auto own_l = [&](int g) { return (sm.red[0][g] + sm.red[1][g]) + (sm.red[2][g] + sm.red[3][g]); };
       // This piece's item starts at flat position `at0` and lies in the shares of CTAs f, f + 1, ..
       const int at0 = w.at - w.c0, f = at0 / share, pieces = (at0 + w.s.chunks - 1) / share - f + 1;
-      bool finish = true;
-      if (pieces > 1) {
+      bf16* to = a.out + w.b * a.ld_o + w.kvh * G * D;
+      if (pieces == 1) {
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float l = own_l(g);
+          if (g < G) to[g * D + r] = f2bf(l > 0.f ? o[g] / l : 0.f);
+        }
+      } else {
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (w.at == begin ? 0 : 1);
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
@@ -528,31 +534,19 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
           if (done == pieces) a.tickets[f] = 0;
         }
         sync_softmax();
-        finish = sm.last;
-      }
-      if (finish) {
-        const int odd = at0 % share ? 1 : 0;  // the first piece is its CTA's last
-#pragma unroll
-        for (int g = 0; g < GP; g += 2) {
-          if (g >= G) break;
-          float m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.f, 0.f}, o2[2] = {0.f, 0.f};
-          if (pieces == 1) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              m2[h] = own_m(g + h);
-              l2[h] = own_l(g + h);
-              o2[h] = o[g + h];
-            }
-          } else {
-            auto slot = [&](int k) { return (2 * static_cast<size_t>(f + k) + (k == 0 ? odd : 0)) * GP + g; };
-            join_parts(
-                m2, l2, o2, pieces,
-                [&](int k, int h) { return reinterpret_cast<const float2*>(a.ws_ml) + slot(k) + h; },
-                [&](int k, int h) { return a.ws_o + (slot(k) + h) * D + r; });
+        if (sm.last) {
+          const int odd = at0 % share ? 1 : 0;  // the first piece is its CTA's last
+#pragma unroll 1
+          for (int g = quarter; g < G; g += 4) {
+            auto at = [&](int k) { return (2 * static_cast<size_t>(f + k) + (k == 0 ? odd : 0)) * GP + g; };
+            const float4 v = join_pieces(
+                pieces, [&](int k) { return reinterpret_cast<const float2*>(a.ws_ml) + at(k); },
+                [&](int k) { return a.ws_o + at(k) * D; });
+            uint2 packed;
+            *reinterpret_cast<bf162*>(&packed.x) = __floats2bfloat162_rn(v.x, v.y);
+            *reinterpret_cast<bf162*>(&packed.y) = __floats2bfloat162_rn(v.z, v.w);
+            *reinterpret_cast<uint2*>(to + g * D + lane * 4) = packed;
           }
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (g + h < G) a.out[w.b * a.ld_o + (w.kvh * G + g + h) * D + r] = f2bf(l2[h] > 0.f ? o2[h] / l2[h] : 0.f);
         }
       }
       sync_softmax();  // red, mrun and last are rewritten by the next piece
