@@ -105,11 +105,11 @@ struct Params {
   const int* seq_lens;
   const int* row_prefix;  // tokens of each row that the prefix kernel has attended to, or null
   bf16* out;
-  const float *prefix_o, *prefix_ml;  // its results (row * Hq + head)
+  const float *prefix_o, *prefix_ml;  // its results, (row * Hq + head) * parts + part
   float *ws_o, *ws_ml;                // [2 * gridDim][Hq / Hkv rounded up to the variant][128] and [..][2]
   int* tickets;                       // [gridDim], zero between launches
   long long ld_o;
-  int max_blocks, blocks, B, Hkv, G, window, sinks;
+  int max_blocks, blocks, B, Hkv, G, parts, window, sinks;
   float scale_log2;
 };
 
@@ -414,15 +414,51 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
       float l_thr[GP], o[GP];
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        float2 ml = make_float2(-INFINITY, 0.f);
-        o[g] = 0.f;
-        if (w.s.prefix && w.c0 == 0 && g < G) {  // the item's first piece goes on from the prefix's result
-          const size_t at = static_cast<size_t>(w.b) * Hq + w.kvh * G + g;
-          ml = *(reinterpret_cast<const float2*>(a.prefix_ml) + at);
-          o[g] = a.prefix_o[at * D + r];
+        if (r == 0) sm.mrun[cur][g] = -INFINITY;
+        l_thr[g] = o[g] = 0.f;
+      }
+      if (w.s.prefix && w.c0 == 0) {
+        // The item's first piece goes on from the prefix's results (read while its
+        // first chunk is on its way).
+        const size_t head = static_cast<size_t>(w.b) * Hq + w.kvh * G;
+        if (a.parts == 1) {  // nothing waits for these loads before the first P V is there
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const size_t at = head + min(g, G - 1);
+            o[g] = a.prefix_o[at * D + r];
+            if (r == 0) {
+              sm.mrun[cur][g] = a.prefix_ml[2 * at];
+              l_thr[g] = a.prefix_ml[2 * at + 1];
+            }
+          }
         }
-        if (r == 0) sm.mrun[cur][g] = ml.x;
-        l_thr[g] = r == 0 ? ml.y : 0.f;
+#pragma unroll
+        for (int g0 = 0; g0 < GP; g0 += 4) {
+          if (a.parts == 1) break;
+          float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int k = 0; k < a.parts; ++k) {
+            float2 ml[4];
+            float op[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const size_t at = (head + min(g0 + g, G - 1)) * a.parts + k;
+              ml[g] = __ldcg(reinterpret_cast<const float2*>(a.prefix_ml) + at);
+              op[g] = __ldcg(a.prefix_o + at * D + r);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float mx = fmaxf(m[g], ml[g].x), ref = mx == -INFINITY ? 0.f : mx;
+              const float w0 = exp2f(m[g] - ref), w1 = exp2f(ml[g].x - ref);
+              o[g0 + g] = o[g0 + g] * w0 + op[g] * w1;
+              l_thr[g0 + g] = r == 0 ? l_thr[g0 + g] * w0 + ml[g].y * w1 : 0.f;
+              m[g] = mx;
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (r == 0) sm.mrun[cur][g0 + g] = m[g];
+        }
       }
       for (int c = w.c0; c < w.c1; ++c, ++cc) {
         if (!mbar_wait(&sm.s_full, cc & 1, FB_KERR_TIMEOUT_TMEM)) *give_up = 1;
@@ -566,10 +602,11 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
   extern "C" __global__ void __launch_bounds__(THREADS, CTAS) fb_span_attn_g##GP(                                 \
       const __grid_constant__ SpanMaps maps, const int* block_tables, int max_blocks, int blocks,                 \
       const int* seq_lens, bf16* out, long long ld_o, int B, int Hkv, int G, int window, int sinks,               \
-      const int* row_prefix, const float* prefix_o, const float* prefix_ml, float* ws_o, float* ws_ml,            \
+      const int* row_prefix, const float* prefix_o, const float* prefix_ml, int parts, float* ws_o, float* ws_ml, \
       int* tickets, float scale_log2) {                                                                           \
-    const Params a{block_tables, seq_lens, row_prefix, out,    prefix_o, prefix_ml, ws_o,   ws_ml, tickets,       \
-                   ld_o,         max_blocks, blocks,   B,      Hkv,      G,         window, sinks, scale_log2};   \
+    const Params a{block_tables, seq_lens, row_prefix, out, prefix_o, prefix_ml, ws_o,   ws_ml,                   \
+                   tickets,      ld_o,     max_blocks, blocks, B,     Hkv,       G,      parts, window,           \
+                   sinks,        scale_log2};                                                                     \
     span_body<GP>(maps, a);                                                                                       \
   }
 

@@ -9,8 +9,9 @@
 //                             of one KV head are the rows of the tile. The
 //                             pages are split over the CTAs of a cluster, which
 //                             join their results through each other's shared
-//                             memory; writes one unnormalised fp32 result and
-//                             (max, sum) per row and head, from which
+//                             memory; writes an unnormalised fp32 result and
+//                             (max, sum) per row and head (a few, where a
+//                             cluster's CTAs are not enough), from which
 //                             attention_span.cu goes on
 //
 // Per key tile and 128-row query tile:
@@ -688,13 +689,13 @@ __device__ __forceinline__ void window_prefill(const CUtensorMap* tmQ, const CUt
 }
 
 // ---- shared prefix of a decode batch ---------------------------------------------------
-// items[blockIdx.x] = {first row, rows, first page, pages}: the rows (sequences)
-// of one group against a range of the pages that its first row's block table
-// begins with; the CTAs of a cluster have the same rows. Row r of query tile t is head r / nb of the group's
+// items[blockIdx.x] = {first row, rows, first page, pages, part}: the rows
+// (sequences) of one group against a range of the pages that its first row's block
+// table begins with; the CTAs of a cluster have the same rows and part. Row r of query tile t is head r / nb of the group's
 // KV head for sequence first + t * nb + r % nb, nb = 128 / G rounded down to a
 // multiple of 8 (whole swizzle atoms), so one TMA box of nb rows fetches one head.
 struct PrefixItem {
-  int row0, rows, page0, pages;
+  int row0, rows, page0, pages, part, pad[3];
 };
 
 template <class Smem>
@@ -704,7 +705,7 @@ struct PrefixWork {
   const int *pages, *seq_lens;
   float *o_part, *ml_part;
   PrefixItem it;
-  int kvh, G, nb, Hq, Hkv, blocks;
+  int kvh, G, nb, Hq, Hkv, parts, blocks;
   int n, sinks;
   static constexpr bool few = false;
   bool more = true;  // a CTA has one item (of no pages, maybe)
@@ -756,7 +757,8 @@ struct PrefixWork {
   // Index of a tile row's result; -1 if no head and sequence uses it.
   __device__ __forceinline__ long long result_of(int t, int r) const {
     const int b = row_of(t, r);
-    return r < G * nb && b < it.rows ? (it.row0 + b) * static_cast<long long>(Hq) + kvh * G + r / nb : -1;
+    if (r >= G * nb || b >= it.rows) return -1;
+    return ((it.row0 + b) * static_cast<long long>(Hq) + kvh * G + r / nb) * parts + it.part;
   }
   static constexpr bool EPILOGUE = false, JOINS = true;
   // O rows of the tiles in the ring's memory, 16-byte chunks swizzled by the row.
@@ -824,8 +826,8 @@ template <class Smem>
 __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const CUtensorMap* tmK,
                                                  const CUtensorMap* tmV, const PrefixItem* items,
                                                  const int* block_tables, int max_blocks, const int* seq_lens,
-                                                 float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks,
-                                                 float scale_log2) {
+                                                 float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts,
+                                                 int blocks, float scale_log2) {
   pdl_wait();
   PrefixWork<Smem> w;
   w.it = items[blockIdx.x];
@@ -841,6 +843,7 @@ __device__ __forceinline__ void prefix_attention(const CUtensorMap* tmQ, const C
   w.nb = (128 / G) & ~7;
   w.Hq = Hq;
   w.Hkv = Hkv;
+  w.parts = parts;
   w.blocks = blocks;
   w.n = (w.it.pages + 1) / 2;
   w.sinks = 0;
@@ -874,13 +877,15 @@ FB_WINDOW_PREFILL(2, 1)
 
 // q [B, Hq * 128] with boxes of nb rows; caches viewed as [blocks * Hkv * 64,
 // 128] with boxes of one page. Grid: (items, Hkv), clusters of the items that
-// share their rows. The result of (row, head) is at index row * Hq + head.
+// share their rows. Part p of the result of (row, head) is at index
+// (row * Hq + head) * parts + p.
 #define FB_PREFIX_ATTN(QT, CTAS)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_prefix_attn_q##QT(                         \
+  extern "C" __global__ void __launch_bounds__(QT == 2 ? 384 : 192, CTAS) fb_prefix_attn_q##QT(                   \
       const __grid_constant__ TileMaps maps, const PrefixItem* items, const int* block_tables, int max_blocks,    \
-      const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int blocks, float scale_log2) {      \
-    prefix_attention<PrefixSmem##QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens, o_part, ml_part,   \
-                         G, Hq, Hkv, blocks, scale_log2);                                                         \
+      const int* seq_lens, float* o_part, float* ml_part, int G, int Hq, int Hkv, int parts, int blocks,          \
+      float scale_log2) {                                                                                         \
+    prefix_attention<PrefixSmem##QT>(&maps.q, &maps.k, &maps.v, items, block_tables, max_blocks, seq_lens,        \
+                                     o_part, ml_part, G, Hq, Hkv, parts, blocks, scale_log2);                     \
   }
 FB_PREFIX_ATTN(1, 2)
 FB_PREFIX_ATTN(2, 1)

@@ -27,7 +27,6 @@ TILE_SMEM = {1: 108 * 1024, 2: 227 * 1024}
 PREFIX_THREADS = {1: 192, 2: 384}  # by query tiles per CTA
 PREFILL_THREADS = {1: 192, 2: 512}
 TILE = 128  # queries (and keys) of a tile
-MAX_CLUSTER = 8  # CTAs that share a prefix's pages between them
 _BF16, _I32 = torch.bfloat16, torch.int32
 
 
@@ -115,7 +114,7 @@ def span_ctas(group: int, sms: int) -> int:
 class SpanWorkspace:
     """Partial results of the decode calls: two pieces per CTA (the same for
     every batch and length), and the results of shared prefixes for
-    ``partials`` (row, head) pairs (``PrefixPlan.partials``). With
+    ``partials`` (row, head, part) results (``PrefixPlan.partials``). With
     ``arena`` the buffers come from it (a runner whose graphs are saved).
 
     Calls that may run at the same time need a workspace each; calls in stream
@@ -159,8 +158,8 @@ def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, d
         # q's heads are a dimension of their own: one box holds a KV head's heads of one row
         q_ptr, 128, n_q, 256, g, b, (q.stride(0) if b > 1 else n_q * 128) * 2,
         block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv, g,
-        window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o_ptr, ws.prefix_ml_ptr, ws.o_ptr,
-        ws.ml_ptr, ws.tickets_ptr, scale * LOG2E, after_own=plan is not None)
+        window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o_ptr, ws.prefix_ml_ptr,
+        plan.parts if plan else 0, ws.o_ptr, ws.ml_ptr, ws.tickets_ptr, scale * LOG2E, after_own=plan is not None)
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -186,13 +185,22 @@ def prefix_rows(group: int) -> int:
     return (128 // group) & ~7
 
 
-def _prefix_splits(tiles: int, pages: int, slots: int) -> int:
-    """CTAs of a cluster that share the ``pages`` of a prefix, for ``tiles``
-    clusters: those with the shortest schedule of ``slots`` CTAs at a time,
-    where a CTA costs its key tiles and about three more for its start and end."""
-    keys = math.ceil(pages / 2)
-    return min((math.ceil(tiles * s / slots) * (math.ceil(keys / s) + 3), s)
-               for s in (1, 2, 4, MAX_CLUSTER) if s <= max(keys, 1))[1]
+# Clusters of c CTAs of fb_prefix_attn_q2 that 148 SMs hold at a time (measured by
+# the second wave's appearance: a cluster lies in one GPC, so not every SM is in
+# one); of fb_prefix_attn_q1, two CTAs per SM, twice as many.
+_CLUSTERS = {1: 148, 2: 72, 3: 44, 4: 32, 5: 24, 6: 16, 7: 14, 8: 13}
+
+
+def _prefix_us(clusters: int, pages: int, tiles: int, cluster: int, parts: int, sms: int) -> float:
+    """Estimated microseconds of the prefix kernel: ``clusters`` (query tiles x KV
+    heads) times ``parts`` clusters of ``cluster`` CTAs, which have an equal part
+    of the pages each. Measured on 148 SMs: 2.1 us per key tile with two query
+    tiles per CTA, 2.2 with two CTAs per SM, 1.8 with one, and 7 us for start,
+    end and join; 0.7 us per further part in the kernel that goes on from them."""
+    held = max(1, _CLUSTERS[cluster] * (3 - tiles) * sms // 148)
+    step = 2.1 if tiles == 2 else 2.2 if clusters * parts * cluster > sms else 1.8
+    keys = math.ceil(math.ceil(pages / 2) / (cluster * parts))
+    return math.ceil(clusters * parts / held) * (keys * step + 7) + 0.7 * (parts - 1)
 
 
 class PrefixPlan:
@@ -203,37 +211,49 @@ class PrefixPlan:
     (0: nothing shared). The lengths need not be known, only that; a row may
     even be shorter than its prefix (a padding row of length 0). The plan
     holds until the batch's composition changes: captured graphs read it, so
-    it has to outlive them."""
+    it has to outlive them.
+
+    Groups that are too small, or prefixes too short, for the shared pages'
+    extra kernel to pay are read row by row (``share=None``: by an estimate of
+    both; True and False decide for it)."""
 
     def __init__(self, group_sizes: list[int], prefix_pages: list[int], n_q: int, n_kv: int, max_blocks: int,
-                 arena=None, device=None):
+                 arena=None, device=None, share: bool | None = None):
         group = _check_group(n_q, n_kv)
         _check(len(group_sizes) == len(prefix_pages), "one number of prefix pages for each group")
         _check(all(n >= 0 for n in group_sizes) and all(0 <= p <= max_blocks for p in prefix_pages),
                f"group sizes must not be negative, prefixes 0 to {max_blocks} pages")
         self.n_q, self.n_kv, self.max_blocks = n_q, n_kv, max_blocks
         self.rows = sum(group_sizes)
-        nb = prefix_rows(group)
-        shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n and p]
-        # two query tiles per CTA as soon as a group has more rows than one
-        self.tiles = 2 if any(n > nb for n, _ in shared) else 1
-        self.kernel = f"fb_prefix_attn_q{self.tiles}"
-        step = nb * self.tiles
-        slots = max(1, _rt.sm_count() * (1 if self.tiles == 2 else 2) // n_kv)
-        clusters = sum(math.ceil(n / step) for n, _ in shared)
-        self.splits = _prefix_splits(clusters, max((p for _, p in shared), default=0), slots)
+        least = 1 if share else 2  # rows that can share anything
+        shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n >= least and p]
+        nb, sms, longest = prefix_rows(group), _rt.sm_count(), max((p for _, p in shared), default=0)
+        us, self.tiles, self.cluster, self.parts = min((
+            (_prefix_us(sum(math.ceil(n / (nb * t)) for n, _ in shared) * n_kv, longest, t, c, p, sms), t, c, p)
+            for t in (1, 2) for c in _CLUSTERS for p in (1, 2, 4, 8) if c * p <= max(1, math.ceil(longest / 2))),
+            default=(0, 1, 1, 1))
+        if share is None:  # row by row at 85% of the HBM rate
+            again = sum(n * p for n, p in shared) * PAGE * n_kv * 512 / 5.5e6
+            share = again > us
+        if not share:
+            shared = []
+        splits = self.cluster * self.parts
         items, info, row = [], [], 0
         for n, pages in zip(group_sizes, prefix_pages):
-            keys = math.ceil(pages / 2)
-            cuts = [min(2 * (keys * s // self.splits), pages) for s in range(self.splits + 1)]
-            if pages:
-                for r0 in range(0, n, step):
-                    items += [[row + r0, min(step, n - r0), a, e - a] for a, e in zip(cuts, cuts[1:])]
-            info += [pages * PAGE] * n
+            is_shared = (n, pages) in shared
+            if is_shared:
+                keys = math.ceil(pages / 2)
+                cuts = [min(2 * (keys * s // splits), pages) for s in range(splits + 1)]
+                for r0 in range(0, n, nb * self.tiles):
+                    items += [[row + r0, min(nb * self.tiles, n - r0), a, e - a, s // self.cluster, 0, 0, 0]
+                              for s, (a, e) in enumerate(zip(cuts, cuts[1:]))]
+            info += [pages * PAGE if is_shared else 0] * n
             row += n
+        self.kernel = f"fb_prefix_attn_q{self.tiles}"
         self.items_n = len(items)
-        self.partials = self.rows * n_q if items else 0  # (row, head) results that a SpanWorkspace has to hold
-        host = torch.tensor(items or [[0] * 4], dtype=_I32), torch.tensor(info or [0], dtype=_I32)
+        # (row, head, part) results that a SpanWorkspace has to hold
+        self.partials = self.rows * n_q * self.parts if items else 0
+        host = torch.tensor(items or [[0] * 8], dtype=_I32), torch.tensor(info or [0], dtype=_I32)
         if arena is not None:
             self.items, self.row_prefix = (arena.empty(tuple(t.shape), _I32) for t in host)
             self.items.copy_(host[0])
@@ -269,7 +289,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0,
             k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0, v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0,
             plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), ws.prefix_o_ptr,
-            ws.prefix_ml_ptr, g, n_q, n_kv, blocks, scale * LOG2E, cluster=plan.splits)
+            ws.prefix_ml_ptr, g, n_q, n_kv, plan.parts, blocks, scale * LOG2E, cluster=plan.cluster)
     _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan if plan.items_n else None)
     return out
 

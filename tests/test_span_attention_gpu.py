@@ -167,12 +167,14 @@ GROUPS = [
     ([5, 1, 2], [3, 0, 1], [192, 200, 0, 150, 321, 90, 64, 130]),  # an empty row, one shorter than its prefix
     ([40, 33], [7, 4], [448 + i for i in range(40)] + [256 + 9 * i for i in range(33)]),
     ([70], [21], [21 * 64 + (i * 7) % 90 for i in range(70)]),
+    ([3, 2], [301, 120], [301 * 64 + 5, 301 * 64, 19_000, 120 * 64 + 64, 1]),  # cut into many parts
 ]
 
 
 @pytest.mark.parametrize("n_q,n_kv", [(4, 1), (8, 8), (6, 2), (32, 8), (10, 2), (32, 4), (16, 1), (28, 2)])
+@pytest.mark.parametrize("share", [True, False])
 @pytest.mark.parametrize("sizes,pages,lens", GROUPS)
-def test_prefix_decode(n_q, n_kv, sizes, pages, lens):
+def test_prefix_decode(n_q, n_kv, sizes, pages, lens, share):
     from foundry_b200 import ops
 
     shared, r = [], 0
@@ -184,7 +186,8 @@ def test_prefix_decode(n_q, n_kv, sizes, pages, lens):
     for r0, n, p in shared:
         ids = table[r0, :p].long()
         kc[ids], vc[ids] = torch.nan_to_num(kc[ids]), torch.nan_to_num(vc[ids])
-    plan = ops.PrefixPlan(sizes, pages, n_q, n_kv, table.shape[1])
+    plan = ops.PrefixPlan(sizes, pages, n_q, n_kv, table.shape[1], share=share)
+    assert bool(plan.items_n) == share
     ws = ops.SpanWorkspace(plan.partials)
     out = torch.full_like(q, 7.0)
     ops.prefix_decode_attention(q, kc, vc, table, lens_t, out, plan, ws)
@@ -204,7 +207,7 @@ def test_prefix_decode_agrees_with_decode_attention_in_a_captured_graph():
     q, kc, vc, table, lens_t = _paged([m + 64 for m in lens], 32, 8, seed=9, shared=[(0, n, pages)])
     lens_t = _i32(lens)
     kc, vc = torch.nan_to_num(kc), torch.nan_to_num(vc)
-    plan = ops.PrefixPlan([n], [pages], 32, 8, table.shape[1])
+    plan = ops.PrefixPlan([n], [pages], 32, 8, table.shape[1], share=True)
     ws = ops.SpanWorkspace(plan.partials)
     out, ref = torch.empty_like(q), torch.empty_like(q)
     dws = ops.DecodeWorkspace(n, 32, 64)
