@@ -42,6 +42,10 @@ class LlamaConfig:
     init_std: float = 0.02
     extra: dict = field(default_factory=dict)
     arch: str = "llama"
+    # sliding-window attention: tokens that a query sees (0: all of them) and first
+    # tokens that stay visible behind the window
+    window: int = 0
+    sinks: int = 0
 
     @property
     def qkv_dim(self) -> int:
@@ -222,9 +226,14 @@ class LlamaModel:
             qkv = self._qkv(st, x, lw, b)
             ops.rope_kv_write(qkv, st.positions[:b], self.cos_sin, st.q[:b], st.k_cache[li], st.v_cache[li],
                               st.slots[:b], w.nq_l, w.nkv_l, lw.get("q_norm"), lw.get("k_norm"), cfg.eps)
-            ops.decode_attention(st.q[:b], st.k_cache[li], st.v_cache[li], st.block_tables[:b], st.seq_lens[:b],
-                                 st.attn_out[:b].view(b, w.nq_l, cfg.head_dim), st.max_pages, st.attn_ws,
-                                 scale=self.scale, splits=splits)
+            attn_out = st.attn_out[:b].view(b, w.nq_l, cfg.head_dim)
+            if cfg.window:
+                ops.window_decode_attention(st.q[:b], st.k_cache[li], st.v_cache[li], st.block_tables[:b],
+                                            st.seq_lens[:b], attn_out, cfg.window, cfg.sinks, st.span_ws,
+                                            scale=self.scale)
+            else:
+                ops.decode_attention(st.q[:b], st.k_cache[li], st.v_cache[li], st.block_tables[:b], st.seq_lens[:b],
+                                     attn_out, st.max_pages, st.attn_ws, scale=self.scale, splits=splits)
             o = self._o_proj(st, st.attn_out[:b], lw, h, b)
             self._norm(st, o, h, lw["mlp_norm"], x, b)
             pending = self._mlp(st, x, h, lw, b)
@@ -324,9 +333,13 @@ class LlamaModel:
                               k_out=pb.k_rot[:t], v_out=pb.v_rot[:t])
             from ..runner.engine import PREFILL_IMPL
 
-            ops.prefill_attention(pb.q[:t].view(t, nqd), pb.k_rot[:t].view(t, nkvd), pb.v_rot[:t].view(t, nkvd),
-                                  pb.attn_out[:t], pb.cu_seqlens, pb.tile_seq, pb.tile_start, w.nq_l, w.nkv_l,
-                                  scale=self.scale, impl=PREFILL_IMPL)
+            qkv_rot = pb.q[:t].view(t, nqd), pb.k_rot[:t].view(t, nkvd), pb.v_rot[:t].view(t, nkvd)
+            if cfg.window:
+                ops.window_prefill_attention(*qkv_rot, pb.attn_out[:t], pb.cu_seqlens[:pb.num_seqs + 1], pb.tile_seq,
+                                             pb.tile_start, w.nq_l, w.nkv_l, cfg.window, cfg.sinks, scale=self.scale)
+            else:
+                ops.prefill_attention(*qkv_rot, pb.attn_out[:t], pb.cu_seqlens, pb.tile_seq, pb.tile_start, w.nq_l,
+                                      w.nkv_l, scale=self.scale, impl=PREFILL_IMPL)
             o = self._o_proj(pb, pb.attn_out[:t], lw, h, t)
             self._norm(pb, o, h, lw["mlp_norm"], x, t)
             pending = self._mlp(pb, x, h, lw, t)
@@ -361,6 +374,16 @@ def _rope(x, pos, cos_sin):
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
+def _hidden(cfg, t_len: int, device) -> torch.Tensor:
+    """[T, T]: the keys that a query does not see."""
+    i = torch.arange(t_len, device=device)
+    back = i[:, None] - i[None]
+    hidden = back < 0
+    if cfg.window:
+        hidden |= (back >= cfg.window) & (i[None] >= cfg.sinks)
+    return hidden
+
+
 def reference_forward(cfg: LlamaConfig, weights: LlamaWeights, ids: torch.Tensor, cos_sin: torch.Tensor,
                       layers: int | None = None) -> torch.Tensor:
     """fp32 causal forward of one sequence; returns logits [T, vocab]."""
@@ -383,8 +406,7 @@ def reference_forward(cfg: LlamaConfig, weights: LlamaWeights, ids: torch.Tensor
         k = k.repeat_interleave(g, dim=1)
         v = v.repeat_interleave(g, dim=1)
         att = torch.einsum("thd,shd->hts", q, k) / math.sqrt(d)
-        mask = torch.triu(torch.ones(t_len, t_len, dtype=torch.bool, device=ids.device), 1)
-        att = att.masked_fill(mask, float("-inf")).softmax(-1)
+        att = att.masked_fill(_hidden(cfg, t_len, ids.device), float("-inf")).softmax(-1)
         o = torch.einsum("hts,shd->thd", att, v).reshape(t_len, cfg.n_q * d)
         h = h + o @ f(lw["o"]).T
         x = _rms(h, f(lw["mlp_norm"]), cfg.eps)

@@ -30,7 +30,7 @@ import torch
 
 from .. import ops
 from ..ops import moe as M
-from .llama import LlamaConfig, LlamaModel, _rms, _rope
+from .llama import LlamaConfig, LlamaModel, _hidden, _rms, _rope
 
 
 @dataclass
@@ -287,8 +287,7 @@ def reference_forward(cfg: Qwen3MoeConfig, weights: Qwen3MoeWeights, ids: torch.
         k = k.repeat_interleave(g, dim=1)
         v = v.repeat_interleave(g, dim=1)
         att = torch.einsum("thd,shd->hts", q, k) / math.sqrt(d)
-        mask = torch.triu(torch.ones(t_len, t_len, dtype=torch.bool, device=ids.device), 1)
-        att = att.masked_fill(mask, float("-inf")).softmax(-1)
+        att = att.masked_fill(_hidden(cfg, t_len, ids.device), float("-inf")).softmax(-1)
         o = torch.einsum("hts,shd->thd", att, v).reshape(t_len, cfg.n_q * d)
         h = h + o @ f(lw["o"]).T
         x = _rms(h, f(lw["mlp_norm"]), cfg.eps)

@@ -30,6 +30,7 @@ from .. import ops
 from ..models import family
 from ..models.llama import LlamaConfig, LlamaWeights
 from ..ops.attention import PREFILL_TILE, DecodeWorkspace, decode_splits, prefill_tiles
+from ..ops.logprobs import MAX_TOP
 from ..ops.gemm import MAX_SPLITS, SWIGLU_SK_ENABLED, PartialBuffer, swiglu_sk_sizes
 from .arena import Arena
 
@@ -167,6 +168,7 @@ class DecodeState:
             b, nq, 1, o_part=arena.empty((cap * 128,), torch.float32),
             ml_part=arena.empty((cap * 2,), torch.float32))
         self.attn_ws.capacity = cap
+        self.span_ws = ops.SpanWorkspace(arena=arena) if cfg.window else None
 
 
 class PrefillBatch:
@@ -223,6 +225,9 @@ class Request:
     prompt: list[int]
     max_new_tokens: int
     output: list[int] = field(default_factory=list)
+    # with log probabilities asked for, of every output token: (log p, entropy of
+    # its distribution, [(token, log p) of the most probable ones])
+    logprobs: list[tuple] = field(default_factory=list)
     row: int = -1            # decode row
     pages: list[int] = field(default_factory=list)
 
@@ -279,6 +284,7 @@ class LLMEngine:
         self.state = DecodeState(ecfg, self.arena, self.k_cache, self.v_cache, self.weights, self.tp, self.ep)
         self.prefill_buf = PrefillBatch(ecfg, self.arena, self.k_cache, self.v_cache, self.weights, self.tp, self.ep)
         self.model = model_cls(cfg, self.weights, self.cos_sin)
+        self._logprob_ws = None  # made when log probabilities are first asked for
         self.graph_sizes = sorted(ecfg.graph_sizes or default_graph_sizes(ecfg.max_batch))
         self.graphs: dict[int, object] = {}
         # Restored graphs share one executable per topology group and patch
@@ -325,8 +331,9 @@ class LLMEngine:
             r.pages, r.row = [], -1
 
     # ---- prefill -------------------------------------------------------------------------------
-    def prefill(self, reqs: list[Request]) -> None:
-        """Prefills requests in packed chunks; appends each request's first token.
+    def prefill(self, reqs: list[Request], logprobs: int | None = None) -> None:
+        """Prefills requests in packed chunks; appends each request's first token
+        (and with ``logprobs`` its log probability and that many alternatives).
         Under expert parallelism every rank runs the same number of chunks
         (padding with one-token chunks) so the exchange steps line up."""
         pb = self.prefill_buf
@@ -345,7 +352,7 @@ class LLMEngine:
 
         with phase("foundry.prefill"):
             for c in chunks:
-                self._prefill_chunk(c)
+                self._prefill_chunk(c, logprobs)
         for _ in range(n - len(chunks)):
             pad = Request(rid=-1, prompt=[0], max_new_tokens=1, pages=[0])
             self._prefill_chunk([pad])
@@ -358,7 +365,7 @@ class LLMEngine:
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         return int(t.item())
 
-    def _prefill_chunk(self, chunk: list[Request]) -> None:
+    def _prefill_chunk(self, chunk: list[Request], logprobs: int | None = None) -> None:
         pb = self.prefill_buf
         off, seqlens = 0, []
         pb.h_cu[0] = 0
@@ -373,7 +380,7 @@ class LLMEngine:
             pb.h_cu[j + 1] = off
             pb.h_last[j] = off - 1
             seqlens.append(n)
-        ts, tst = prefill_tiles(seqlens, PREFILL_TILE[PREFILL_IMPL])
+        ts, tst = prefill_tiles(seqlens, 128 if self.ecfg.model.window else PREFILL_TILE[PREFILL_IMPL])
         pb.h_tile_seq[:len(ts)] = torch.tensor(ts, dtype=torch.int32)
         pb.h_tile_start[:len(ts)] = torch.tensor(tst, dtype=torch.int32)
         n_seq = len(chunk)
@@ -397,6 +404,21 @@ class LLMEngine:
         pb.h_next[:n_seq].copy_(pb.next_ids[:n_seq])
         for j, r in enumerate(chunk):
             r.output.append(int(pb.h_next[j]))
+        if logprobs is not None:
+            for r, lp in zip(chunk, self._logprobs(pb.logits[:n_seq], pb.next_ids[:n_seq], logprobs)):
+                r.logprobs.append(lp)
+
+    def _logprobs(self, logits: torch.Tensor, ids: torch.Tensor, k: int) -> list[tuple]:
+        """(log p, entropy, [(token, log p)] * k) of each row's token."""
+        n = ids.numel()
+        if self._logprob_ws is None:
+            self._logprob_ws = ops.LogprobWorkspace(device=self.device)
+        f32 = {"dtype": torch.float32, "device": self.device}
+        lp, entropy, top = torch.empty(n, **f32), torch.empty(n, **f32), torch.empty(n, k, **f32)
+        top_ids = torch.empty(n, k, dtype=torch.int32, device=self.device)
+        ops.token_logprobs(logits, ids, lp, entropy, top, top_ids, ws=self._logprob_ws)
+        return [(p, h, list(zip(t, v))) for p, h, t, v in
+                zip(lp.tolist(), entropy.tolist(), top_ids.tolist(), top.tolist())]
 
     # ---- decode --------------------------------------------------------------------------------
     def bucket(self, n: int) -> int:
@@ -455,19 +477,38 @@ class LLMEngine:
             self.model.decode(st, b)
 
     def generate(self, prompts: list[list[int]], max_new_tokens: int) -> list[list[int]]:
+        return [r.output for r in self._generate(prompts, max_new_tokens, None)]
+
+    def generate_logprobs(self, prompts: list[list[int]], max_new_tokens: int,
+                          top: int = 0) -> tuple[list[list[int]], list[list[tuple]]]:
+        """``generate``, and for every token (log p, entropy of its distribution,
+        [(token, log p)] of the ``top`` most probable ones). Not for a
+        vocabulary sharded over tensor-parallel ranks."""
+        if self.tp is not None:
+            raise ValueError("log probabilities need the whole vocabulary on this rank (tp = 1)")
+        if not 0 <= top <= min(MAX_TOP, self.weights.vocab_l):
+            raise ValueError(f"top must be 0 to {min(MAX_TOP, self.weights.vocab_l)}, got {top}")
+        reqs = self._generate(prompts, max_new_tokens, top)
+        return [r.output for r in reqs], [r.logprobs for r in reqs]
+
+    def _generate(self, prompts: list[list[int]], max_new_tokens: int, logprobs: int | None) -> list[Request]:
         reqs = self.add_requests(prompts, max_new_tokens)
-        self.prefill(reqs)
+        self.prefill(reqs, logprobs)
         b = self.start_decode(reqs)
         steps = max_new_tokens - 1
         if self.ep is not None:  # every rank takes the same decode steps (and graph sizes stay per rank)
             steps = self._max_over_ranks(steps)
         for _ in range(steps):
             toks = self.decode_step(b)
+            if logprobs is not None:
+                lps = self._logprobs(self.state.logits[:b], self.state.next_ids[:b], logprobs)
             for r in reqs:
                 if not r.done:
                     r.output.append(int(toks[r.row]))
+                    if logprobs is not None:
+                        r.logprobs.append(lps[r.row])
         self.release(reqs)
-        return [r.output for r in reqs]
+        return reqs
 
     # ---- graphs --------------------------------------------------------------------------------
     def warmup(self) -> None:
