@@ -207,7 +207,7 @@ __device__ __forceinline__ float4 join_pieces(int n, Ml ml, Part part) {
     }
     m = mx;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros; NaN stays NaN
   return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -553,7 +553,7 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           const float l = own_l(g);
-          if (g < G) to[g * D + r] = f2bf(l > 0.f ? o[g] / l : 0.f);
+          if (g < G) to[g * D + r] = f2bf(l == 0.f ? 0.f : o[g] / l);
         }
       } else {
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (w.at == begin ? 0 : 1);

@@ -356,6 +356,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
     const uint32_t t_s = tmem + t * 128 + lane_base, t_o = tmem + (QT + t) * 128 + lane_base;
     uint32_t tiles = 0, items = 0;
     bool ok = true;
+    w.begin(t);
 #pragma unroll 1
     for (; ok && w.next(); ++items) {
       int hi, lo;
@@ -419,9 +420,10 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           }
         }
         if (t == 0 && w.zero_row(i, r)) {
-          // A key row behind the prompt's end holds another prompt's values or
-          // nothing at all, and 0 * NaN = NaN: its V row is zeroed once the copy
-          // has landed (tile 0's P V runs first, so once is enough).
+          // A key that no row sees (behind the prompt's end, or every row's) holds
+          // another prompt's values or nothing at all, and 0 * NaN = NaN: its V row
+          // is zeroed once the copy has landed (tile 0's P V runs first, so once is
+          // enough).
           const uint32_t at = 2 * tiles + 1, slot = at % SLOTS;
           if (!mbar_wait(&sm.kv_full[slot], (at / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
           uint8_t* vrow = sm.kv[slot] + r * 128;
@@ -603,6 +605,7 @@ struct WindowWork {
   __device__ __forceinline__ int key0(int i) const { return (i < n_sink ? i : i - n_sink + first) * BK; }
   __device__ __forceinline__ bool zero_row(int i, int r) const { return key0(i) + r >= s1 - s0; }
   __device__ __forceinline__ void clear_q(Smem&) const {}
+  __device__ __forceinline__ void begin(int) const {}
   __device__ __forceinline__ void load_q(Smem& sm, uint64_t* bar, int t) const {
     mbar_arrive_expect_tx(bar, TILE);
     for (int h = 0; h < 2; ++h) tma_load_2d(sm.q[t] + h * HALF, tmQ, bar, (head0 + t) * D + h * 64, s0 + qp0);
@@ -626,7 +629,7 @@ struct WindowWork {
   template <class Read>
   __device__ __forceinline__ void store(Smem& sm, int t, int r, uint32_t t_o, float, float l, Read read) const {
     constexpr int CHUNKS = Smem::STAGE / 16, ROWS = 32 / CHUNKS;  // chunks of a staged row; rows of a store
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // (NaN stays NaN)
     const int lane = r & 31, row0 = s0 + qp0 + (r & ~31), my_row = lane / CHUNKS, my_chunk = lane % CHUNKS;
     uint8_t* stage = sm.stage[r >> 5];
     auto at = [&](int row, int chunk) {
@@ -716,7 +719,17 @@ struct PrefixWork {
   }
 
   __device__ __forceinline__ int key0(int i) const { return it.page0 * PAGE + i * BK; }
-  __device__ __forceinline__ bool zero_row(int, int) const { return false; }
+  int longest;  // of the item's rows, in query tile 0's softmax warps (which look for it while the first K is on its way)
+  __device__ __forceinline__ void begin(int t) {
+    if (t != 0) return;
+    int n_keys = 0;
+    for (int b = threadIdx.x & 31; b < it.rows; b += 32) n_keys = max(n_keys, seq_lens[it.row0 + b]);
+    longest = __reduce_max_sync(0xffffffffu, n_keys);
+  }
+  __device__ __forceinline__ bool zero_row(int i, int r) const {
+    const int key = key0(i) + r;
+    return key >= longest && key < (it.page0 + it.pages) * PAGE;  // (TMA has filled what is behind with zeros)
+  }
   // Rows that no head and sequence uses hold zeros and see every key: what
   // they compute is finite and dropped, and keeps no warp on the masked path.
   __device__ __forceinline__ void clear_q(Smem& sm) const {
@@ -736,11 +749,14 @@ struct PrefixWork {
   __device__ __forceinline__ void load_kv(uint8_t* dst, uint64_t* bar, int i, int v) const {
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-      // a tile's second page behind the end: rows past the cache, which TMA fills with zeros
-      int page = 2 * i + pg < it.pages ? pages[it.page0 + 2 * i + pg] : blocks;
-      if (page < 0 || page > blocks) {
-        set_status(FB_KERR_BAD_ARG);
-        page = blocks;
+      // No page (a tile's second one behind the end): rows past the cache, which TMA fills with zeros.
+      int page = blocks;
+      if (2 * i + pg < it.pages) {
+        page = pages[it.page0 + 2 * i + pg];
+        if (page < 0 || page >= blocks) {
+          set_status(FB_KERR_BAD_ARG);
+          page = blocks;
+        }
       }
       const int row = (page * Hkv + kvh) * PAGE;
       for (int h = 0; h < 2; ++h)
@@ -808,7 +824,7 @@ struct PrefixWork {
 #pragma unroll
       for (int c = 0; c < MAX_CLUSTER; ++c) {
         const float e = exp2f(ml[c].x - ref);
-        if (!(e > 0.f)) continue;  // (an empty part's O is no number)
+        if (ml[c].y == 0.f) continue;  // (an empty part's O is no number)
         l = fmaf(ml[c].y, e, l);
         sum.x = fmaf(o[c].x, e, sum.x);
         sum.y = fmaf(o[c].y, e, sum.y);

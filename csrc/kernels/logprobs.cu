@@ -4,8 +4,8 @@
 // With y = (x - max) log2(e), Z = sum 2^y, U = sum 2^y y:
 //   log p(t) = x_t - max - ln Z        H = ln Z - U ln 2 / Z
 // (both terms of H are >= 0, so nothing cancels). Each thread keeps its own
-// running max and rescales (Z, U) when it moves, once per 32 bytes at most; Z
-// and U are fp32 sums of at most a few hundred terms each, joined as a tree.
+// running max and rescales (Z, U) when it moves, once per 64 bytes at most; Z
+// and U are fp32 sums: of the 64 bytes, of those, then a tree over the threads.
 //
 // The k largest (ties: lowest token) come from the same pass: each thread also
 // knows the max of what it has read. The block's 256 threads make 64 groups,
@@ -179,7 +179,7 @@ struct Smem {
   float group_max[GROUPS];
   unsigned char listed[THREADS];  // threads whose max reaches the bound
   int n_listed;
-  Sums sums[WARPS], total;
+  Sums sums[WARPS];
   unsigned long long best[MAX_K];
   unsigned long long key;
   unsigned bound;  // ordered bits
@@ -509,7 +509,8 @@ __device__ __forceinline__ void logprobs_body(const Params& a) {
       const float mx = Vec<T>::max_of(raw);
       tmax = fmaxf(tmax, mx);
       if (mx > s.ref) s.move(mx);
-      float2 z2 = make_float2(s.z, 0.f), u2 = make_float2(s.u, 0.f);
+      // (Sums of their own: a term far below Z is not lost one by one in rounding Z.)
+      float2 z2 = make_float2(0.f, 0.f), u2 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         if (q >= count) break;
@@ -520,8 +521,8 @@ __device__ __forceinline__ void logprobs_body(const Params& a) {
       }
       const float u = u2.x + u2.y;
       if (u == u) {
-        s.z = z2.x + z2.y;
-        s.u = u;
+        s.z += z2.x + z2.y;
+        s.u += u;
         return;
       }
 #pragma unroll 1

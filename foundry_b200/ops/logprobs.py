@@ -68,13 +68,13 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
     if logits.dim() != 2 or logits.dtype not in _NAMES or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise ValueError("logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
     t, v = logits.shape
-    if not 0 < v < 1 << 30:
-        raise ValueError(f"vocabulary of {v}")
+    if not 0 < v < 1 << 30 or t >= 1 << 30:
+        raise ValueError(f"{t} rows of a vocabulary of {v}")
     if (top_logprobs is None) != (top_ids is None) or (ids is None) != (logprobs is None):
         raise ValueError("top_logprobs and top_ids come together, and ids and logprobs")
     k = 0
     if top_ids is not None:
-        k = top_ids.shape[-1]
+        k = top_ids.shape[-1] if top_ids.dim() else 0
         if k > min(MAX_TOP, v):
             raise ValueError(f"at most {min(MAX_TOP, v)} alternatives, got {k}")
     cur = torch.cuda.current_device()

@@ -79,8 +79,8 @@ def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int,
                 and k_cache.get_device() == cur and v_cache.get_device() == cur and out.get_device() == cur
                 and block_tables.get_device() == cur and seq_lens.get_device() == cur
                 and (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15 == 0
-                and blocks > 0 and max_blocks > 0 and (blocks + 1) * n_kv * PAGE < 1 << 31
-                and b * n_kv * (max_blocks // 2 + 2) < 1 << 31):
+                and blocks > 0 and 0 < max_blocks <= 1 << 24 and (blocks + 1) * n_kv * PAGE < 1 << 31
+                and b * n_kv * (max_blocks // 2 + 2) < 1 << 30):
             return b, n_q, n_kv, blocks, max_blocks
     _check(q.dim() == 3 and q.shape[2] == 128 and q.dtype == _BF16, "q must be bf16 [batch, heads, 128]")
     b, n_q, _ = q.shape
@@ -101,7 +101,7 @@ def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int,
     _check(seq_lens.dtype == _I32 and tuple(seq_lens.shape) == (b,) and seq_lens.is_contiguous(),
            "seq_lens must be contiguous int32 [batch]")
     max_blocks = block_tables.shape[1]
-    _check(0 < max_blocks and b * n_kv * (max_blocks // 2 + 2) < 1 << 31, "block_tables of no or too many pages")
+    _check(0 < max_blocks <= 1 << 24 and b * n_kv * (max_blocks // 2 + 2) < 1 << 30, "block_tables of no or too many pages")
     _check_device(q, k_cache, v_cache, block_tables, seq_lens, out)
     return b, n_q, n_kv, blocks, max_blocks
 
@@ -235,12 +235,10 @@ class PrefixPlan:
         if share is None:  # row by row at 85% of the HBM rate
             again = sum(n * p for n, p in shared) * PAGE * n_kv * 512 / 5.5e6
             share = again > us
-        if not share:
-            shared = []
         splits = self.cluster * self.parts
         items, info, row = [], [], 0
         for n, pages in zip(group_sizes, prefix_pages):
-            is_shared = (n, pages) in shared
+            is_shared = share and n >= least and pages > 0
             if is_shared:
                 keys = math.ceil(pages / 2)
                 cuts = [min(2 * (keys * s // splits), pages) for s in range(splits + 1)]
@@ -314,7 +312,7 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         ld, inner = x.stride()
         if t == 1:
             ld = heads * 128
-        if inner != 1 or ld % 8 or ld < heads * 128 or x.data_ptr() % 16:
+        if inner != 1 or ld % 8 or not heads * 128 <= ld < 1 << 30 or x.data_ptr() % 16:
             raise ValueError("q, k, v and out must be row-contiguous with 16-byte aligned rows that do not overlap")
         maps += x.data_ptr(), heads * 128, t, ld * 2, TILE, 0, 0
     for x in (cu_seqlens, tile_seq, tile_start):
@@ -332,6 +330,6 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     _rt.launch_mapped(
         _TILE, "fb_window_prefill_q2" if qt == 2 else "fb_window_prefill_q1",
         min(n_tiles * (n_q // qt), _rt.sm_count() * (3 - qt)), 1, PREFILL_THREADS[qt], TILE_SMEM[qt], 3, *maps[:21],
-        out.data_ptr(), out.stride(0), t, n_seqs, cu_seqlens.data_ptr(), tile_seq.data_ptr(), tile_start.data_ptr(),
+        out.data_ptr(), ld, t, n_seqs, cu_seqlens.data_ptr(), tile_seq.data_ptr(), tile_start.data_ptr(),
         n_tiles, n_q, n_kv, window, sinks, scale * LOG2E)
     return out

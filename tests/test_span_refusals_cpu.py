@@ -238,3 +238,33 @@ def test_logprob_shares_cover_every_logit_once(rows, vocab):
         if len(got) > 1:
             for i, (_, _, _, is_first) in enumerate(got):
                 assert is_first == (not (i == 0 and row * pitch % share))
+
+
+def test_sizes_that_indices_do_not_hold_are_refused(launches):
+    """On tensors without that memory behind them (expanded ones, or none at all)."""
+    bf = dict(dtype=torch.bfloat16, device="meta")
+    a = {k: v.to("meta") for k, v in _decode().items()}
+    a["block_tables"] = torch.empty(3, (1 << 24) + 1, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="too many pages"):
+        S._decode_dims(*a.values())
+    a["block_tables"] = torch.empty(1 << 22, 1 << 9, dtype=torch.int32, device="meta")
+    a["q"] = a["out"] = torch.empty(1 << 22, 8, 128, **bf)
+    a["seq_lens"] = torch.empty(1 << 22, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="too many pages"):
+        S._decode_dims(*a.values())
+    a = {k: v.to("meta") for k, v in _decode().items()}
+    a["k_cache"] = a["v_cache"] = torch.empty(1 << 24, 2, 64, 128, **bf)
+    with pytest.raises(ValueError, match="too many blocks"):
+        S._decode_dims(*a.values())
+    with pytest.raises(ValueError, match="rows of a vocabulary"):
+        ops.token_logprobs(torch.zeros(1, 1).expand(1 << 30, 1), None, None, None, ws=ops.LogprobWorkspace(device="cpu"))
+    far = torch.empty(1, dtype=torch.bfloat16, device="meta").as_strided((200, 512), (1 << 31, 1))
+    with pytest.raises(ValueError, match="do not overlap"):
+        ops.window_prefill_attention(*{**_prefill(), "out": far}.values(), 4, 2, 64, 4)
+    assert not launches
+
+
+def test_a_plan_of_many_groups_is_made_at_once():
+    n = 20_000
+    p = ops.PrefixPlan([2] * n, [4] * n, 8, 2, 8, device="cpu", share=True)
+    assert p.items_n == n * p.cluster * p.parts
