@@ -58,13 +58,15 @@ struct Smem {
   uint8_t p[QP_BYTES];
   uint64_t kfull, vfull, kempty, vempty;
   uint64_t s_full, s_empty, p_full, o_full, o_empty;
-  float red[4][NH];    // per-warp max, then per-warp sum, of every head
+  float red_max[4][NH], red_sum[4][NH];  // of a warp's tokens, for every head
   float mrun[2][NH];   // running max per head: one in use, one for the next move
   int scan[THREADS / 32];
   int first_row, first_off;
   int2 first_length;
   uint32_t tmem;
-  int last;
+  struct {
+    int f, pieces, odd, b, kvh, last;
+  } cut[2];  // the pieces of items that lie in other CTAs' shares too: at most the first and the last one
   int abort;
   int give_up;  // a softmax thread's wait ran out: read by all of them between the same two barriers
 };
@@ -408,6 +410,8 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const int G = a.G, Hq = a.Hkv * G;
     uint32_t cc = 0;
+    int cuts = 0;
+    bool stop = false;
     int cur = 0;  // which of mrun is in use (the same in all threads)
     volatile int* give_up = &sm.give_up;
     for (Walk w(a, sm, begin, end); w.more(); w.next(a)) {
@@ -471,18 +475,6 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
         if (lane == 0) mbar_arrive(&sm.s_empty);
         const int vp = 2 * c + (r >> 6), tok = w.s.page(vp) * PAGE + (r & 63);
         const bool valid = vp < w.s.pages && tok < w.s.n && (tok >= w.s.lo || tok < w.s.sinks);
-        if (!valid) {
-          // The P V product reads all 128 rows of V: those that no token is
-          // visible in hold stale or never-written memory, and 0 * NaN = NaN,
-          // so they are zeroed once this chunk's V copies have landed.
-          if (!mbar_wait(&sm.vfull, cc & 1, FB_KERR_TIMEOUT_FULL)) *give_up = 1;
-          uint8_t* vrow = sm.v + r * 128;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              reinterpret_cast<uint4*>(vrow + h * HALF_STRIDE)[i] = make_uint4(0, 0, 0, 0);
-        }
         // The maxima move only if a score is above one by more than 8 (log2
         // units: p stays below 256, exact in the fp32 sums), and in a piece's
         // first chunk: the reduction over the tokens is for those chunks alone.
@@ -493,38 +485,69 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
           sr[g] = __float_as_uint(s);
           move |= g < G && c > w.c0 && s > sm.mrun[cur][g] + 8.f;
         }
-        move = sync_softmax_or(move);
-        if (*give_up) break;  // the same in every softmax thread: written only outside this pair of barriers
+        if (c > w.c0) {
+          move = sync_softmax_or(move);
+          if ((stop = *give_up)) break;  // the same in every softmax thread: written only outside this pair of barriers
+        }
         if (move) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
             const float cmax = warp_max(__uint_as_float(sr[g]));
-            if (lane == 0) sm.red[quarter][g] = cmax;
+            if (lane == 0) sm.red_max[quarter][g] = cmax;
           }
           sync_softmax();
+          if (c == w.c0 && (stop = *give_up)) break;  // (as above)
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
-            const float mx = fmaxf(fmaxf(sm.red[0][g], sm.red[1][g]), fmaxf(sm.red[2][g], sm.red[3][g]));
+            const float mx =
+                fmaxf(fmaxf(sm.red_max[0][g], sm.red_max[1][g]), fmaxf(sm.red_max[2][g], sm.red_max[3][g]));
             const float m_old = sm.mrun[cur][g], m_new = fmaxf(m_old, mx);
             const float alpha = exp2f(m_old - (m_new == -INFINITY ? 0.f : m_new));
             if (r == 0) sm.mrun[cur ^ 1][g] = m_new;
+            sr[g] = __float_as_uint(__uint_as_float(sr[g]) - (m_new == -INFINITY ? 0.f : m_new));
             l_thr[g] *= alpha;
             o[g] *= alpha;
           }
           cur ^= 1;
-          sync_softmax();  // mrun is read below
+        } else {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float m = sm.mrun[cur][g];
+            sr[g] = __float_as_uint(__uint_as_float(sr[g]) - (m == -INFINITY ? 0.f : m));
+          }
         }
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float m = sm.mrun[cur][g];
-          const float p = exp2f(__uint_as_float(sr[g]) - (m == -INFINITY ? 0.f : m));
+          const float p = exp2f(__uint_as_float(sr[g]));
           l_thr[g] += p;
           if (g < G) *reinterpret_cast<bf16*>(sm.p + qp_offset(g, r)) = f2bf(p);
+        }
+        bool late = false;
+        if (!valid) {
+          // The P V product reads all 128 rows of V: those that no token is
+          // visible in hold stale or never-written memory, and 0 * NaN = NaN,
+          // so they are zeroed once this chunk's V copies have landed. (Each
+          // lane from its own 16 bytes on: a warp's lanes in different banks.)
+          late = !mbar_wait(&sm.vfull, cc & 1, FB_KERR_TIMEOUT_FULL);
+          uint8_t* vrow = sm.v + r * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(vrow + h * HALF_STRIDE)[i ^ (r & 7)] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
         sync_softmax();
         if (lane == 0) mbar_arrive(&sm.p_full);
-        if (!mbar_wait(&sm.o_full, cc & 1, FB_KERR_TIMEOUT_TMEM)) *give_up = 1;
+        if (c + 1 == w.c1) {  // the heads' sums over the token lanes, while P V is on its way
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float ls = warp_sum(l_thr[g]);
+            if (lane == 0) sm.red_sum[quarter][g] = ls;
+          }
+          sync_softmax();
+        }
+        if (late || !mbar_wait(&sm.o_full, cc & 1, FB_KERR_TIMEOUT_TMEM)) *give_up = 1;
         tc_fence_after();
         uint32_t orr[GP];
         tmem_ld_cols<GP>(t_o + lane_base, orr);
@@ -535,24 +558,15 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
 #pragma unroll
         for (int g = 0; g < GP; ++g) o[g] += __uint_as_float(orr[g]);
       }
-      // Sum of a head over the 128 token lanes.
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        const float ls = warp_sum(l_thr[g]);
-        if (lane == 0) sm.red[quarter][g] = ls;
-      }
-      sync_softmax();
-      if (*give_up) break;  // again the same in every thread; the workspace's tickets are then left as they are
-      // Every thread of the piece's heads: their max and sum (the same in all), its dim of their outputs.
-      auto own_m = [&](int g) { return sm.mrun[cur][g]; };
-      auto own_l = [&](int g) { return (sm.red[0][g] + sm.red[1][g]) + (sm.red[2][g] + sm.red[3][g]); };
-      // This piece's item starts at flat position `at0` and lies in the shares of CTAs f, f + 1, ..
-      const int at0 = w.at - w.c0, f = at0 / share, pieces = (at0 + w.s.chunks - 1) / share - f + 1;
-      bf16* to = a.out + w.b * a.ld_o + w.kvh * G * D;
-      if (pieces == 1) {
+      if (stop) break;
+      auto sum = [&](int g) {
+        return (sm.red_sum[0][g] + sm.red_sum[1][g]) + (sm.red_sum[2][g] + sm.red_sum[3][g]);
+      };
+      if (w.c0 == 0 && w.c1 == w.s.chunks) {
+        bf16* to = a.out + w.b * a.ld_o + w.kvh * G * D;
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float l = own_l(g);
+          const float l = sum(g);
           if (g < G) to[g * D + r] = f2bf(l == 0.f ? 0.f : o[g] / l);
         }
       } else {
@@ -560,34 +574,47 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           __stcg(a.ws_o + (slot * GP + g) * D + r, o[g]);
-          if (r == 0) __stcg(reinterpret_cast<float2*>(a.ws_ml) + slot * GP + g, make_float2(own_m(g), own_l(g)));
+          if (r == 0) __stcg(reinterpret_cast<float2*>(a.ws_ml) + slot * GP + g, make_float2(sm.mrun[cur][g], sum(g)));
         }
-        sync_softmax();
         if (r == 0) {
-          // releases the warps' writes (ordered before it by the barrier), acquires the other pieces'
-          const int done = add_acq_rel(a.tickets + f, 1) + 1;
-          sm.last = done == pieces;
-          if (done == pieces) a.tickets[f] = 0;
+          // The item starts at flat position `at0` and lies in the shares of CTAs f, f + 1, ..;
+          // odd: its first piece is its CTA's last.
+          const int at0 = w.at - w.c0, f = at0 / share;
+          sm.cut[cuts] = {f, (at0 + w.s.chunks - 1) / share - f + 1, at0 % share ? 1 : 0, w.b, w.kvh, 0};
         }
-        sync_softmax();
-        if (sm.last) {
-          const int odd = at0 % share ? 1 : 0;  // the first piece is its CTA's last
+        ++cuts;
+      }
+    }
+    // Cut items, last: by now the first piece's results have long been written, and
+    // nothing has had to wait for that.
+    sync_softmax();
+    if (*give_up) {  // the workspace's tickets are left as they are
+      sm.abort = 1;
+    } else if (cuts) {
+      if (lane == 0 && quarter < cuts) {
+        // releases the warps' writes (ordered before it by the barrier), acquires the other pieces'
+        auto& cut = sm.cut[quarter];
+        const int done = add_acq_rel(a.tickets + cut.f, 1) + 1;
+        cut.last = done == cut.pieces;
+        if (done == cut.pieces) a.tickets[cut.f] = 0;
+      }
+      sync_softmax();
+      for (int i = 0; i < cuts; ++i) {
+        const auto cut = sm.cut[i];
+        if (!cut.last) continue;
 #pragma unroll 1
-          for (int g = quarter; g < G; g += 4) {
-            auto at = [&](int k) { return (2 * static_cast<size_t>(f + k) + (k == 0 ? odd : 0)) * GP + g; };
-            const float4 v = join_pieces(
-                pieces, [&](int k) { return reinterpret_cast<const float2*>(a.ws_ml) + at(k); },
-                [&](int k) { return a.ws_o + at(k) * D; });
-            uint2 packed;
-            *reinterpret_cast<bf162*>(&packed.x) = __floats2bfloat162_rn(v.x, v.y);
-            *reinterpret_cast<bf162*>(&packed.y) = __floats2bfloat162_rn(v.z, v.w);
-            *reinterpret_cast<uint2*>(to + g * D + lane * 4) = packed;
-          }
+        for (int g = quarter; g < G; g += 4) {
+          auto at = [&](int k) { return (2 * static_cast<size_t>(cut.f + k) + (k == 0 ? cut.odd : 0)) * GP + g; };
+          const float4 v = join_pieces(
+              cut.pieces, [&](int k) { return reinterpret_cast<const float2*>(a.ws_ml) + at(k); },
+              [&](int k) { return a.ws_o + at(k) * D; });
+          uint2 packed;
+          *reinterpret_cast<bf162*>(&packed.x) = __floats2bfloat162_rn(v.x, v.y);
+          *reinterpret_cast<bf162*>(&packed.y) = __floats2bfloat162_rn(v.z, v.w);
+          *reinterpret_cast<uint2*>(a.out + cut.b * a.ld_o + (cut.kvh * G + g) * D + lane * 4) = packed;
         }
       }
-      sync_softmax();  // red, mrun and last are rewritten by the next piece
     }
-    if (*give_up) sm.abort = 1;
   }
 
   tc_fence_before();

@@ -428,8 +428,8 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           if (!mbar_wait(&sm.kv_full[slot], (at / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
           uint8_t* vrow = sm.kv[slot] + r * 128;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          for (int e = 0; e < 16; ++e)  // (each lane from its own 16 bytes on: a warp's lanes in different banks)
+            *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF + ((e ^ r) & 7) * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
