@@ -191,6 +191,9 @@ def prefix_rows(group: int) -> int:
 _CLUSTERS = {1: 148, 2: 72, 3: 44, 4: 32, 5: 24, 6: 16, 7: 14, 8: 13}
 
 
+_PREFIX_LEAST_US = 7.0  # of the prefix kernel: start, end and join
+
+
 def _prefix_us(clusters: int, pages: int, tiles: int, cluster: int, parts: int, sms: int) -> float:
     """Estimated microseconds of the prefix kernel: ``clusters`` (query tiles x KV
     heads) times ``parts`` clusters of ``cluster`` CTAs, which have an equal part
@@ -199,8 +202,8 @@ def _prefix_us(clusters: int, pages: int, tiles: int, cluster: int, parts: int, 
     end and join; 0.7 us per further part in the kernel that goes on from them."""
     held = max(1, _CLUSTERS[cluster] * (3 - tiles) * sms // 148)
     step = 2.1 if tiles == 2 else 2.2 if clusters * parts * cluster > sms else 1.8
-    keys = math.ceil(math.ceil(pages / 2) / (cluster * parts))
-    return math.ceil(clusters * parts / held) * (keys * step + 7) + 0.7 * (parts - 1)
+    keys = -(-((pages + 1) // 2) // (cluster * parts))
+    return -(-clusters * parts // held) * (keys * step + _PREFIX_LEAST_US) + 0.7 * (parts - 1)
 
 
 class PrefixPlan:
@@ -228,13 +231,15 @@ class PrefixPlan:
         least = 1 if share else 2  # rows that can share anything
         shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n >= least and p]
         nb, sms, longest = prefix_rows(group), _rt.sm_count(), max((p for _, p in shared), default=0)
-        us, self.tiles, self.cluster, self.parts = min((
-            (_prefix_us(sum(math.ceil(n / (nb * t)) for n, _ in shared) * n_kv, longest, t, c, p, sms), t, c, p)
-            for t in (1, 2) for c in _CLUSTERS for p in (1, 2, 4, 8) if c * p <= max(1, math.ceil(longest / 2))),
-            default=(0, 1, 1, 1))
-        if share is None:  # row by row at 85% of the HBM rate
-            again = sum(n * p for n, p in shared) * PAGE * n_kv * 512 / 5.5e6
-            share = again > us
+        us, self.tiles, self.cluster, self.parts = 0.0, 1, 1, 1
+        again = sum(n * p for n, p in shared) * PAGE * n_kv * 512 / 5.5e6  # us row by row, at 85% of the HBM rate
+        if shared and (share or share is None and again > _PREFIX_LEAST_US):
+            us, self.tiles, self.cluster, self.parts = min(
+                (_prefix_us(clusters, longest, t, c, p, sms), t, c, p)
+                for t, clusters in ((t, n_kv * sum(-(-n // (nb * t)) for n, _ in shared)) for t in (1, 2))
+                for c in _CLUSTERS for p in (1, 2, 4, 8) if c * p <= max(1, (longest + 1) // 2))
+        if share is None:
+            share = again > max(us, _PREFIX_LEAST_US)
         splits = self.cluster * self.parts
         items, info, row = [], [], 0
         for n, pages in zip(group_sizes, prefix_pages):
@@ -251,14 +256,14 @@ class PrefixPlan:
         self.items_n = len(items)
         # (row, head, part) results that a SpanWorkspace has to hold
         self.partials = self.rows * n_q * self.parts if items else 0
-        host = torch.tensor(items or [[0] * 8], dtype=_I32), torch.tensor(info or [0], dtype=_I32)
+        host = torch.tensor([x for item in items or [[0] * 8] for x in item] + (info or [0]), dtype=_I32)
         if arena is not None:
-            self.items, self.row_prefix = (arena.empty(tuple(t.shape), _I32) for t in host)
-            self.items.copy_(host[0])
-            self.row_prefix.copy_(host[1])
+            on_device = arena.empty(tuple(host.shape), _I32)
+            on_device.copy_(host)
         else:
-            device = device or torch.device("cuda", torch.cuda.current_device())
-            self.items, self.row_prefix = (t.to(device) for t in host)
+            on_device = host.to(device or torch.device("cuda", torch.cuda.current_device()))
+        n = 8 * max(1, len(items))
+        self.items, self.row_prefix = on_device[:n].view(-1, 8), on_device[n:]
 
 
 def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
