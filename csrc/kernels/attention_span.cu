@@ -4,7 +4,7 @@
 //
 //   window > 0:  [0, min(sinks, n)) and [max(n - window, 0), n)
 //   window = 0:  [start, n), start = the tokens that fb_prefix_attn_* has
-//                attended to for the whole group (row_info)
+//                attended to for the whole group (row_prefix)
 //
 // Pages without a visible token are never touched; of a page that is visible
 // in part, only the 16-token blocks with a visible token are read.
@@ -30,6 +30,14 @@
 // Single 64 KB stage per CTA and three CTAs per SM (two for more than eight
 // heads per KV head, by registers): K and V have their own barriers, so the
 // next chunk's K loads during this chunk's softmax and P V.
+//
+// Measured (B200), K and V of the visible tokens over the time: 256 rows of 1024
+// tokens, 32 / 8 heads 168 us (97% of the 6545 GB/s of a plain copy); 61 rows of
+// 4160 tokens, 32 / 4 heads 88 us (89%); 256 rows of 1 to 640 tokens 63 us (81%);
+// 1024 rows of 64 tokens 57 us (72%); one row of 1028 tokens 9.2 us. A launch's
+// start (lengths, page numbers, first K) and end (last chunk, join) take 6 to 9 us;
+// between them a full chunk's chain is hidden by the other CTAs' loads, a row of
+// one chunk takes 3.9 k clocks of a CTA.
 //
 // Roles: warp 0 TMA producer, warp 1 TMEM owner + MMA issuer, warps 2..5
 // softmax and epilogue. No TMA multicast. All waits bounded (fb_common.cuh).

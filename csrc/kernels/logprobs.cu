@@ -24,12 +24,16 @@
 // copies its next 128 bytes into its own slots of shared memory while it works on
 // 64, which takes neither registers nor barriers. (Slower: loads ahead into
 // registers, which spill; a ring of bulk copies for the block, whose barriers cost
-// as many instructions as the sums do.) Up to as many rows as CTAs, a row has a whole number of
-// CTAs, so that no CTA ends two rows; beyond, the flat sequence of all logits is
-// cut into one equal share per CTA. A row that a cut falls into is joined by the CTA
-// that finishes its last piece, through a workspace of two pieces per CTA and
-// one ticket per cut (zero before and after every launch). The join is in
-// piece order, so results do not depend on which CTA comes last.
+// as many instructions as the sums do.) Up to as many rows as CTAs, a row has a
+// whole number of CTAs, so that no CTA ends two rows; beyond, the flat sequence of
+// all logits is cut into one equal share per CTA. A row that a cut falls into is
+// joined by the CTA that finishes its last piece, through a workspace of two pieces
+// per CTA and one ticket per cut (zero before and after every launch). The join is
+// in piece order, so results do not depend on which CTA comes last.
+//
+// Measured (B200): 2000 x 151936 fp32, k = 1 197 us (94% of the 6545 GB/s of a plain
+// copy), bf16 125 us (74%); 256 x 128256 bf16, k = 0 / 5 / 20 16.7 / 19.2 / 21.3 us
+// (3.9 / 3.4 / 3.1 TB/s: two rows on most SMs, 1.73 on average); one row, k = 5 8.7 us.
 #include <cuda_fp16.h>
 
 #include "fb_common.cuh"

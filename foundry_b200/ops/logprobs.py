@@ -42,7 +42,9 @@ class LogprobWorkspace:
 def share_of(rows: int, vocab: int, ctas: int) -> tuple[int, int]:
     """(logits per CTA, flat distance of two rows). Up to ``ctas`` rows, each
     has a whole number of CTAs of its own; more rows are one flat sequence cut
-    into equal shares."""
+    into equal shares. (256 rows of 128256 on 444 CTAs, k = 0 / 5 / 20: 16.7 /
+    19.2 / 21.2 us so, 19.9 / 25.8 / 48.2 us in equal shares, whose CTAs end two
+    rows each.)"""
     if rows <= ctas:
         parts = max(1, min(ctas // rows, vocab // MIN_SHARE))
         share = math.ceil(vocab / parts / 64) * 64

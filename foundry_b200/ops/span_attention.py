@@ -304,8 +304,9 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     """Causal attention over packed prompts with a sliding window and sinks.
     q: [T, *] with head h at columns h * 128 (row stride q.stride(0)); k, v
     likewise with n_kv heads; out [T, n_q * 128]. The tile tables come from
-    ``prefill_tiles(seqlens)``. Rows outside every prompt are neither used
-    (they may hold anything) nor written."""
+    ``prefill_tiles(seqlens)``; a tile that starts behind its prompt's end is
+    skipped (padding). Rows outside every prompt are neither used (they may hold
+    anything) nor written."""
     group = _check_group(n_q, n_kv)
     _check_window(window, sinks)
     scale = _check_scale(scale)
