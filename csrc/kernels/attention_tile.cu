@@ -50,7 +50,7 @@
 // Bound by the chain of a step rather than by a pipe: softmax 1900 clocks, signal
 // to the MMA warp 440, P V and the next Q K^T 1020; two query tiles overlap their
 // chains (the tensor pipe is busy 55% of a long prompt's 3700-clock steps), TMEM
-// has no room for a third. Slower or within 2%: P handed over in halves; 1 in 2, 1 in
+// has no room for a third. Slower or within 2%: two threads per row; P handed over in halves; 1 in 2, 1 in
 // 3 or no exponentials by polynomial; masks block by block; skipping masked
 // blocks of 32 keys.
 // No TMA multicast; every wait bounded (fb_common.cuh).
