@@ -19,6 +19,7 @@ HOOK_LIB = LIB_DIR / "libfoundry_hook.so"
 MOCK_DRIVER = LIB_DIR / "libfoundry_mockcuda.so"
 
 _C = None
+_tensors = None
 
 
 def core():
@@ -33,6 +34,20 @@ def core():
                 f"(or __graft_entry__.build()): {e}"
             ) from e
     return _C
+
+
+def tensors():
+    """The module of the short ops' tensor checks (csrc/tensors), importing it on first use."""
+    global _tensors
+    if _tensors is None:
+        try:
+            _tensors = importlib.import_module("foundry_b200._tensors")
+        except ImportError as e:
+            raise ImportError(
+                "foundry_b200._tensors is not built; run `python -m foundry_b200._build` "
+                f"(or __graft_entry__.build()): {e}"
+            ) from e
+    return _tensors
 
 
 def use_mock_driver() -> None:

@@ -94,17 +94,19 @@ def launch(image: str, name: str, grid, block, args, smem: int = 0, stream: int 
 
 
 def launch_mapped(image: str, name: str, grid_x: int, grid_y: int, threads: int, smem: int, n_maps: int, *numbers,
-                  cluster: int = 1, after_own: bool = False) -> None:
+                  device: int | None = None, cluster: int = 1, after_own: bool = False) -> None:
     """``launch`` on the current stream for ops whose calls are short: numbers
     only, ``n_maps`` times 7 of them for the tensor maps that the kernel takes
-    as its first parameter (csrc/core/module.cpp), then its arguments.
+    as its first parameter (csrc/core/module.cpp), then its arguments. ``device``:
+    the current one, if the caller has asked for it already.
 
     ``after_own``: the launch right before it on this stream is one of the
     same op; this kernel may be set up while that one runs (it waits for it
     before it reads anything, as every kernel of ``PDL_IMAGES`` does)."""
     fn = _funcs.get((image, name, smem)) or function(image, name, smem)
-    core().launch_mapped(fn, grid_x, grid_y, threads, smem,
-                         torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()), cluster,
+    if device is None:
+        device = torch.cuda.current_device()
+    core().launch_mapped(fn, grid_x, grid_y, threads, smem, torch._C._cuda_getCurrentRawStream(device), cluster,
                          PDL_ENABLED and (after_own or getattr(_pdl, "depth", 0) > 0), n_maps, *numbers)
 
 

@@ -7,6 +7,7 @@ import math
 
 import torch
 
+from .. import _native as native
 from . import _rt
 
 _IMG = "logprobs"
@@ -14,7 +15,8 @@ MAX_TOP = 32
 CTAS_PER_SM = 3
 SMEM = 75 * 1024
 MIN_SHARE = 4096  # logits per CTA: below it the join of a row's pieces costs more than it saves
-_NAMES = {torch.bfloat16: "fb_logprobs_bf16", torch.float16: "fb_logprobs_f16", torch.float32: "fb_logprobs_f32"}
+_KINDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NAMES = ("fb_logprobs_bf16", "fb_logprobs_f16", "fb_logprobs_f32")
 
 
 class LogprobWorkspace:
@@ -34,6 +36,7 @@ class LogprobWorkspace:
         self.keys = empty((2 * self.ctas * MAX_TOP,), torch.int64)
         self.tickets = zeros((self.ctas,), torch.int32)
         self.sums_ptr, self.keys_ptr, self.tickets_ptr = self.sums.data_ptr(), self.keys.data_ptr(), self.tickets.data_ptr()
+        self.device = self.tickets.get_device()
 
     def clear(self) -> None:
         self.tickets.zero_()
@@ -67,21 +70,35 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
     type's lowest value; a row that is -inf throughout, or holds +inf or NaN,
     gives NaN (its ``top_ids`` are the order of its logits, NaN left out and -1
     for what is missing)."""
-    if logits.dim() != 2 or logits.dtype not in _NAMES or (logits.stride(1) != 1 and logits.shape[1] != 1):
+    cur = torch.cuda.current_device()
+    numbers = native.tensors().rows(logits, ids, logprobs, entropy, top_logprobs, top_ids, cur)
+    if numbers is None:  # not what almost every call is
+        numbers = _look(logits, ids, logprobs, entropy, top_logprobs, top_ids, cur)
+    kind, t, v, k, ld, x, *outs = numbers
+    if k > MAX_TOP or k > v:
+        raise ValueError(f"at most {min(MAX_TOP, v)} alternatives, got {k}")
+    if ws.device != cur:
+        raise ValueError(f"the workspace must be on the current CUDA device {cur}")
+    if not t:
+        return
+    share, pitch = share_of(t, v, ws.ctas)
+    _rt.launch_mapped(
+        _IMG, _NAMES[kind], min(ws.ctas, -(-t * pitch // share)), 1, 256, SMEM, 0, x, ld, *outs, ws.sums_ptr,
+        ws.keys_ptr, ws.tickets_ptr, share, pitch, t, v, k, device=cur)
+
+
+def _look(logits, ids, logprobs, entropy, top_logprobs, top_ids, cur: int) -> tuple[int, ...]:
+    """(kind of logits, rows, vocabulary, alternatives, row stride, addresses) of a call, or a ValueError."""
+    if logits.dim() != 2 or logits.dtype not in _KINDS or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise ValueError("logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
     t, v = logits.shape
     if not 0 < v < 1 << 30 or t >= 1 << 30:
         raise ValueError(f"{t} rows of a vocabulary of {v}")
     if (top_logprobs is None) != (top_ids is None) or (ids is None) != (logprobs is None):
         raise ValueError("top_logprobs and top_ids come together, and ids and logprobs")
-    k = 0
-    if top_ids is not None:
-        k = top_ids.shape[-1] if top_ids.dim() else 0
-        if k > min(MAX_TOP, v):
-            raise ValueError(f"at most {min(MAX_TOP, v)} alternatives, got {k}")
-    cur = torch.cuda.current_device()
-    if logits.get_device() != cur or ws.tickets.get_device() != cur:
-        raise ValueError(f"logits and workspace must be on the current CUDA device {cur}")
+    k = top_ids.shape[-1] if top_ids is not None and top_ids.dim() else 0
+    if logits.get_device() != cur:
+        raise ValueError(f"logits must be on the current CUDA device {cur}")
     ptrs = []
     for x, dtype, shape in ((ids, torch.int32, (t,)), (logprobs, torch.float32, (t,)), (entropy, torch.float32, (t,)),
                             (top_logprobs, torch.float32, (t, k)), (top_ids, torch.int32, (t, k))):
@@ -91,9 +108,4 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, logprobs: tor
         if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.get_device() != cur:
             raise ValueError(f"expected contiguous {dtype} {shape} on device {cur}, got {x.dtype} {tuple(x.shape)} on {x.device}")
         ptrs.append(x.data_ptr())
-    if not t:
-        return
-    share, pitch = share_of(t, v, ws.ctas)
-    _rt.launch_mapped(
-        _IMG, _NAMES[logits.dtype], min(ws.ctas, math.ceil(t * pitch / share)), 1, 256, SMEM, 0, logits.data_ptr(),
-        logits.stride(0), *ptrs, ws.sums_ptr, ws.keys_ptr, ws.tickets_ptr, share, pitch, t, v, k)
+    return _KINDS[logits.dtype], t, v, k, logits.stride(0), logits.data_ptr(), *ptrs

@@ -17,6 +17,7 @@ import math
 
 import torch
 
+from .. import _native as native
 from . import _rt
 from .attention import LOG2E, PAGE
 
@@ -62,26 +63,13 @@ def _check_group(n_q: int, n_kv: int) -> int:
     return n_q // n_kv
 
 
-def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int, int, int, int, int]:
-    """(batch, n_q, n_kv, blocks, max_blocks) of a decode call, or a ValueError."""
-    if q.dim() == 3 and k_cache.dim() == 4 and block_tables.dim() == 2:
-        # What almost every call is, seen with few questions; anything else is looked at one by one.
-        b, n_q, d = q.shape
-        blocks, n_kv, page, _ = shape = k_cache.shape
-        max_blocks = block_tables.shape[1]
-        cur = torch.cuda.current_device()
-        if (d == 128 and page == PAGE and shape[3] == 128 and q.dtype is _BF16 and k_cache.dtype is _BF16
-                and v_cache.dtype is _BF16 and out.dtype is _BF16 and block_tables.dtype is _I32
-                and seq_lens.dtype is _I32 and out.shape == q.shape and v_cache.shape == shape
-                and block_tables.shape[0] == b and seq_lens.shape == (b,) and q.is_contiguous()
-                and out.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
-                and block_tables.is_contiguous() and seq_lens.is_contiguous() and q.get_device() == cur
-                and k_cache.get_device() == cur and v_cache.get_device() == cur and out.get_device() == cur
-                and block_tables.get_device() == cur and seq_lens.get_device() == cur
-                and (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15 == 0
-                and blocks > 0 and 0 < max_blocks <= 1 << 24 and (blocks + 1) * n_kv * PAGE < 1 << 31
-                and b * n_kv * (max_blocks // 2 + 2) < 1 << 30):
-            return b, n_q, n_kv, blocks, max_blocks
+def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int, ...]:
+    """(batch, n_q, n_kv, blocks, max_blocks, the tensors' addresses, row strides
+    of q and out, device) of a decode call, or a ValueError."""
+    cur = torch.cuda.current_device()
+    numbers = native.tensors().decode(q, k_cache, v_cache, block_tables, seq_lens, out, cur, PAGE)
+    if numbers is not None:  # what almost every call is; anything else is looked at one by one
+        return *numbers, cur
     _check(q.dim() == 3 and q.shape[2] == 128 and q.dtype == _BF16, "q must be bf16 [batch, heads, 128]")
     b, n_q, _ = q.shape
     _check(out.shape == q.shape and out.dtype == _BF16, "out must be bf16 of q's shape")
@@ -103,7 +91,9 @@ def _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out) -> tuple[int,
     max_blocks = block_tables.shape[1]
     _check(0 < max_blocks <= 1 << 24 and b * n_kv * (max_blocks // 2 + 2) < 1 << 30, "block_tables of no or too many pages")
     _check_device(q, k_cache, v_cache, block_tables, seq_lens, out)
-    return b, n_q, n_kv, blocks, max_blocks
+    ld = n_q * 128
+    return (b, n_q, n_kv, blocks, max_blocks, *(t.data_ptr() for t in (q, k_cache, v_cache, block_tables, seq_lens, out)),
+            *(t.stride(0) if b > 1 else ld for t in (q, out)), cur)
 
 
 def span_ctas(group: int, sms: int) -> int:
@@ -129,6 +119,7 @@ class SpanWorkspace:
             empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
             zeros = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
         self.sms = _rt.sm_count()
+        self.ctas = [span_ctas(g, self.sms) for g in range(MAX_GROUP + 1)]  # of a launch, by heads per KV head
         pieces = max(2 * span_ctas(g, self.sms) * p for g, p in ((8, 8), (16, 16)))  # (piece, head) pairs
         self.o = empty((pieces * 128,), torch.float32)
         self.ml = empty((pieces * 2,), torch.float32)
@@ -138,28 +129,28 @@ class SpanWorkspace:
         self.prefix_ml = empty((max(partials, 1) * 2,), torch.float32)
         self.o_ptr, self.ml_ptr, self.tickets_ptr = self.o.data_ptr(), self.ml.data_ptr(), self.tickets.data_ptr()
         self.prefix_o_ptr, self.prefix_ml_ptr = self.prefix_o.data_ptr(), self.prefix_ml.data_ptr()
+        self.device = self.tickets.get_device()
 
     def clear(self) -> None:
         self.tickets.zero_()
 
 
-def _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws: SpanWorkspace, dims, window: int, sinks: int,
-          scale: float, plan: "PrefixPlan | None" = None) -> None:
-    b, n_q, n_kv, blocks, max_blocks = dims
-    g = n_q // n_kv
-    k, v, rows, q_ptr = k_cache.data_ptr(), v_cache.data_ptr(), blocks * n_kv * PAGE, q.data_ptr()
-    if ws.tickets.get_device() != q.get_device():
+def _span(dims, ws: SpanWorkspace, window: int, sinks: int, scale: float, plan: "PrefixPlan | None" = None) -> None:
+    b, n_q, n_kv, blocks, max_blocks, q, k, v, tables, lens, out, ld_q, ld_out, device = dims
+    g, rows = n_q // n_kv, blocks * n_kv * PAGE
+    if ws.device != device:
         raise ValueError("the workspace is on another device")
     _rt.launch_mapped(
         _SPAN, "fb_span_attn_g4" if g <= 4 else "fb_span_attn_g8" if g <= 8 else "fb_span_attn_g16",
-        min(span_ctas(g, ws.sms), b * n_kv * (max_blocks // 2 + 2)), 1, 192, SPAN_SMEM, 5,
+        min(ws.ctas[g], b * n_kv * (max_blocks // 2 + 2)), 1, 192, SPAN_SMEM, 5,
         k, 128, rows, 256, PAGE, 0, 0, v, 128, rows, 256, PAGE, 0, 0, k, 128, rows, 256, 16, 0, 0,
         v, 128, rows, 256, 16, 0, 0,
         # q's heads are a dimension of their own: one box holds a KV head's heads of one row
-        q_ptr, 128, n_q, 256, g, b, (q.stride(0) if b > 1 else n_q * 128) * 2,
-        block_tables.data_ptr(), max_blocks, blocks, seq_lens.data_ptr(), out.data_ptr(), out.stride(0), b, n_kv, g,
-        window, sinks, plan.row_prefix.data_ptr() if plan else 0, ws.prefix_o_ptr, ws.prefix_ml_ptr,
-        plan.parts if plan else 0, ws.o_ptr, ws.ml_ptr, ws.tickets_ptr, scale * LOG2E, after_own=plan is not None)
+        q, 128, n_q, 256, g, b, ld_q * 2,
+        tables, max_blocks, blocks, lens, out, ld_out, b, n_kv, g,
+        window, sinks, plan.row_prefix_ptr if plan else 0, ws.prefix_o_ptr, ws.prefix_ml_ptr,
+        plan.parts if plan else 0, ws.o_ptr, ws.ml_ptr, ws.tickets_ptr, scale * LOG2E, device=device,
+        after_own=plan is not None)
 
 
 def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -176,7 +167,7 @@ def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     _check_window(window, sinks)
     scale = _check_scale(scale)
     if dims[0]:
-        _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, window, sinks, scale)
+        _span(dims, ws, window, sinks, scale)
     return out
 
 
@@ -264,6 +255,8 @@ class PrefixPlan:
             on_device = host.to(device or torch.device("cuda", torch.cuda.current_device()))
         n = 8 * max(1, len(items))
         self.items, self.row_prefix = on_device[:n].view(-1, 8), on_device[n:]
+        self.items_ptr, self.row_prefix_ptr = self.items.data_ptr(), self.row_prefix.data_ptr()
+        self.device = on_device.get_device()
 
 
 def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -274,7 +267,8 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     result and the arguments are those of ``decode_attention`` (``seq_lens``
     counts all tokens, ``block_tables`` begin with the shared pages). Rows of
     length 0 get zeros."""
-    dims = b, n_q, n_kv, blocks, max_blocks = _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out)
+    dims = _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out)
+    b, n_q, n_kv, blocks, max_blocks, q_ptr, k, v, tables, lens, _, ld_q, _, device = dims
     if (plan.rows, plan.n_q, plan.n_kv, plan.max_blocks) != (b, n_q, n_kv, max_blocks):
         raise ValueError(f"plan for {plan.rows} rows, {plan.n_q} / {plan.n_kv} heads and {plan.max_blocks} pages, "
                          f"got {b}, {n_q} / {n_kv} and {max_blocks}")
@@ -283,17 +277,17 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     scale = _check_scale(scale)
     if not b:
         return out
-    if plan.items.get_device() != q.get_device() or ws.tickets.get_device() != q.get_device():
+    if plan.device != device or ws.device != device:
         raise ValueError("the plan or the workspace is on another device")
     if plan.items_n:
         g, rows = n_q // n_kv, blocks * n_kv * PAGE
         _rt.launch_mapped(
             _TILE, plan.kernel, plan.items_n, n_kv, PREFIX_THREADS[plan.tiles], TILE_SMEM[plan.tiles], 3,
-            q.data_ptr(), n_q * 128, b, (q.stride(0) if b > 1 else n_q * 128) * 2, prefix_rows(g), 0, 0,
-            k_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0, v_cache.data_ptr(), 128, rows, 256, PAGE, 0, 0,
-            plan.items.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), ws.prefix_o_ptr,
-            ws.prefix_ml_ptr, g, n_q, n_kv, plan.parts, blocks, scale * LOG2E, cluster=plan.cluster)
-    _span(q, k_cache, v_cache, block_tables, seq_lens, out, ws, dims, 0, 0, scale, plan if plan.items_n else None)
+            q_ptr, n_q * 128, b, ld_q * 2, prefix_rows(g), 0, 0,
+            k, 128, rows, 256, PAGE, 0, 0, v, 128, rows, 256, PAGE, 0, 0,
+            plan.items_ptr, tables, max_blocks, lens, ws.prefix_o_ptr,
+            ws.prefix_ml_ptr, g, n_q, n_kv, plan.parts, blocks, scale * LOG2E, device=device, cluster=plan.cluster)
+    _span(dims, ws, 0, 0, scale, plan if plan.items_n else None)
     return out
 
 
