@@ -268,3 +268,67 @@ def test_a_plan_of_many_groups_is_made_at_once():
     n = 20_000
     p = ops.PrefixPlan([2] * n, [4] * n, 8, 2, 8, device="cpu", share=True)
     assert p.items_n == n * p.cluster * p.parts
+
+
+class _NoTensors:
+    """The detailed checks alone."""
+
+    decode = rows = staticmethod(lambda *a: None)
+
+
+def test_native_checks_agree_with_the_detailed_ones(launches, monkeypatch):
+    a, ws, lws = _decode(b=5, n_q=24, n_kv=3), _ws(partials=1 << 12), ops.LogprobWorkspace(device="cpu")
+    plan = ops.PrefixPlan([5], [2], 24, 3, 4, device="cpu", share=True)
+    x, f, i = torch.zeros(5, 90), torch.zeros(5), torch.zeros(5, dtype=torch.int32)
+    top, top_ids = torch.zeros(5, 7), torch.zeros(5, 7, dtype=torch.int32)
+
+    def calls():
+        launches.clear()
+        _window(a, ws=ws)
+        ops.prefix_decode_attention(*a.values(), plan, ws)
+        for dtype in (torch.bfloat16, torch.float16, torch.float32):
+            ops.token_logprobs(x.to(dtype), i, f, f, top, top_ids, ws=lws)
+        ops.token_logprobs(x[:, 3:80], None, None, f, ws=lws)
+        ops.token_logprobs(x[:, :1], i, f, None, ws=lws)
+        # without the address of a temporary
+        return [(args[:7] if args[0] == "logprobs" else args, kw, args[8:]) for args, kw in launches]
+
+    got = calls()
+    assert len(got) == 8
+    monkeypatch.setattr(S.native, "tensors", lambda: _NoTensors)
+    assert calls() == got
+
+
+def test_native_checks_leave_other_calls_to_the_detailed_ones():
+    n = S.native.tensors()
+    a = list(_decode().values())
+    assert n.decode(*a, -1, 64)[:5] == (3, 8, 2, 10, 4) and n.decode(*a, 0, 64) is None
+    for at, other in ((0, torch.zeros(3, 8, 136, dtype=torch.bfloat16)[..., :128]), (0, None), (1, a[1][:, :1]),
+                      (1, a[1].float()), (3, a[3].long()), (4, a[4][:2]), (5, a[5].unsqueeze(0)), (4, 7)):
+        assert n.decode(*a[:at], other, *a[at + 1:], -1, 64) is None
+    assert n.decode(*a, -1, 32) is None
+    x, f, i = torch.zeros(3, 9), torch.zeros(3), torch.zeros(3, dtype=torch.int32)
+    assert n.rows(x, i, f, None, None, None, -1)[:5] == (2, 3, 9, 0, 9)
+    for args in ((None, i, f, f, None, None), (x.t(), None, None, f, None, None), (x, i, None, f, None, None),
+                 (x, i.long(), f, f, None, None), (x, i, f, f, f, i), (x.double(), i, f, f, None, None)):
+        assert n.rows(*args, -1) is None
+    for bad in ((), (1, 2), tuple(a)):
+        with pytest.raises(TypeError):
+            n.decode(*bad)
+
+
+def test_workspace_or_plan_of_another_device_is_refused(launches):
+    a, ws, lws = _decode(), _ws(partials=1 << 10), ops.LogprobWorkspace(device="cpu")
+    plan = ops.PrefixPlan([3], [2], 8, 2, 4, device="cpu", share=True)
+    ws.device = 1
+    with pytest.raises(ValueError, match="another device"):
+        _window(a, ws=ws)
+    with pytest.raises(ValueError, match="another device"):
+        ops.prefix_decode_attention(*a.values(), plan, ws)
+    ws.device, plan.device = -1, 1
+    with pytest.raises(ValueError, match="another device"):
+        ops.prefix_decode_attention(*a.values(), plan, ws)
+    lws.device = 1
+    with pytest.raises(ValueError, match="current CUDA device"):
+        ops.token_logprobs(torch.zeros(2, 5), None, None, torch.zeros(2), ws=lws)
+    assert not launches
