@@ -14,6 +14,7 @@ sequences grow.
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -52,9 +53,15 @@ def _check_scale(scale: float | None) -> float:
     return float(scale)
 
 
-def _check_window(window: int, sinks: int) -> None:
+def _check_window(window: int, sinks: int) -> tuple[int, int]:
+    """As plain integers: a float among a launch's numbers reaches the kernel as its bits."""
+    try:
+        window, sinks = operator.index(window), operator.index(sinks)
+    except TypeError:
+        raise ValueError(f"window and sinks must be whole numbers, got {window!r}, {sinks!r}") from None
     if not (0 < window < 1 << 30 and 0 <= sinks < 1 << 30):
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window}, {sinks}")
+    return window, sinks
 
 
 def _check_group(n_q: int, n_kv: int) -> int:
@@ -164,7 +171,7 @@ def window_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     pages may have been freed. Rows of length 0 get zeros."""
     dims = _decode_dims(q, k_cache, v_cache, block_tables, seq_lens, out)
     _check_group(dims[1], dims[2])
-    _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks)
     scale = _check_scale(scale)
     if dims[0]:
         _span(dims, ws, window, sinks, scale)
@@ -302,7 +309,7 @@ def window_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     skipped (padding). Rows outside every prompt are neither used (they may hold
     anything) nor written."""
     group = _check_group(n_q, n_kv)
-    _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks)
     scale = _check_scale(scale)
     maps = []
     t = q.shape[0]

@@ -1,0 +1,48 @@
+"""Numbers of the windowed, shared-prefix and log-probability calls that are not
+whole: refused where a whole number is meant, on the CPU with the launch
+replaced by one that records its numbers."""
+
+import numpy as np
+import pytest
+import torch
+
+from foundry_b200 import ops
+from foundry_b200.ops import _rt
+
+
+@pytest.fixture(autouse=True)
+def launches(monkeypatch):
+    got = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)  # what get_device() says of a CPU tensor
+    monkeypatch.setattr(_rt, "sm_count", lambda: 148)
+    monkeypatch.setattr(_rt, "launch_mapped", lambda *a, **k: got.append(a))
+    return got
+
+
+def _decode(window, sinks):
+    bf = dict(dtype=torch.bfloat16)
+    cache = torch.zeros(10, 2, 64, 128, **bf)
+    q, lens = torch.zeros(3, 8, 128, **bf), torch.ones(3, dtype=torch.int32)
+    ops.window_decode_attention(q, cache, cache, torch.zeros(3, 4, dtype=torch.int32), lens, torch.zeros_like(q),
+                                window, sinks, ops.SpanWorkspace(device="cpu"))
+
+
+def _prefill(window, sinks):
+    q, kv = torch.zeros(200, 512, dtype=torch.bfloat16), torch.zeros(200, 256, dtype=torch.bfloat16)
+    tiles = torch.tensor([0, 128], dtype=torch.int32)
+    ops.window_prefill_attention(q, kv, kv, torch.zeros_like(q), torch.tensor([0, 200], dtype=torch.int32),
+                                 torch.zeros_like(tiles), tiles, 4, 2, window, sinks)
+
+
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_window_and_sinks_are_whole_numbers(launches, call):
+    """As a float they would reach the kernel's integers as their bits: a window over everything."""
+    for window, sinks in ((1024.0, 4), (64.5, 4), (64, 4.0), (np.float32(64), 0), ("64", 0), (None, 0), (64, None)):
+        with pytest.raises(ValueError, match="window"):
+            call(window, sinks)
+    assert not launches
+    for window, sinks in ((64, 4), (np.int64(64), np.int32(4)), (torch.tensor(64), torch.tensor(4))):
+        call(window, sinks)
+        numbers = launches.pop()[2:]
+        assert sum(isinstance(x, float) for x in numbers) == 1  # the scale
+        assert all(type(x) in (int, float) for x in numbers) and {64, 4} <= set(numbers)
