@@ -221,6 +221,10 @@ class PrefixPlan:
     def __init__(self, group_sizes: list[int], prefix_pages: list[int], n_q: int, n_kv: int, max_blocks: int,
                  arena=None, device=None, share: bool | None = None):
         group = _check_group(n_q, n_kv)
+        try:
+            group_sizes, prefix_pages = ([operator.index(x) for x in v] for v in (group_sizes, prefix_pages))
+        except TypeError:
+            raise ValueError(f"group sizes and prefix pages must be whole numbers, got {group_sizes}, {prefix_pages}") from None
         _check(len(group_sizes) == len(prefix_pages), "one number of prefix pages for each group")
         _check(all(n >= 0 for n in group_sizes) and all(0 <= p <= max_blocks for p in prefix_pages),
                f"group sizes must not be negative, prefixes 0 to {max_blocks} pages")

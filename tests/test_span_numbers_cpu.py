@@ -46,3 +46,14 @@ def test_window_and_sinks_are_whole_numbers(launches, call):
         numbers = launches.pop()[2:]
         assert sum(isinstance(x, float) for x in numbers) == 1  # the scale
         assert all(type(x) in (int, float) for x in numbers) and {64, 4} <= set(numbers)
+
+
+def test_plan_takes_whole_rows_and_pages():
+    """2.5 pages would be 160 tokens that the rows leave out, of which the shared kernel reads 128."""
+    for sizes, pages in (([3], [2.5]), ([3], [2.0]), ([3.0], [2]), ([1.5, 1.5], [2, 2]), ([3], ["2"]), ([None], [2])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            ops.PrefixPlan(sizes, pages, 8, 2, 4, device="cpu", share=True)
+    want = ops.PrefixPlan([3, 2], [2, 4], 8, 2, 4, device="cpu", share=True)
+    for sizes, pages in ((np.array([3, 2]), np.array([2, 4])), (torch.tensor([3, 2]), torch.tensor([2, 4]))):
+        plan = ops.PrefixPlan(sizes, pages, 8, 2, 4, device="cpu", share=True)
+        assert plan.rows == 5 and torch.equal(plan.items, want.items) and torch.equal(plan.row_prefix, want.row_prefix)
