@@ -105,9 +105,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -116,11 +116,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // take time for; some on the FMA pipes bring the softmax below the products.
 // x = n + f, |f| <= 1/2; 2^f by the polynomial of degree 4 with the least relative
 // error (2.7e-6, found by linear programming; p is rounded to 2^-9 next). x below
-// -126 gives 2^-126 at least.
+// -126 gives 2^-126 at least, and so does NaN: the caller sees to it that the sum
+// of a row with such a score is NaN.
 constexpr int POLY_OF = 4;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = max_nan(x.x, -126.f);
-  x.y = max_nan(x.y, -126.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
   const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f);
   const float2 t = __fadd2_rn(x, magic);  // the low bits are n
   const float2 n = __fadd2_rn(t, unmagic);
@@ -449,10 +450,12 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 128; c += 2)
-          mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-        const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale_log2;
-        const float m_new = mx > m_run + RESCALE_LOG2 || m_run == -INFINITY ? fmaxf(m_run, mx) : m_run;
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          mx4[(c >> 1) & 3] = max3_nan(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        const float mx = max_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale_log2;
+        const float m_new = mx <= m_run + RESCALE_LOG2 ? m_run : max_nan(m_run, mx);  // (from -inf it always moves)
+        // A NaN score makes the maximum NaN, and an infinite one what is subtracted
+        // here (inf - inf): all p of the row and its sum are then NaN.
+        const float m_use = m_new == -INFINITY ? 0.f : fmaf(m_new, 0.f, m_new);
         const float alpha = exp2f(m_run - m_use);  // 1 unless the max moved; 0 while nothing was seen
         if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
