@@ -86,8 +86,8 @@ struct Smem {
   float l[QT][STAGE && QT == 2 ? BQ : 1];  // the rows' sums for the epilogue
   uint64_t q_full[QT], q_empty[QT], kv_full[SLOTS], kv_empty[SLOTS];
   uint64_t s_full[QT], p_full[QT], o_full[QT], l_full[QT], o_empty[QT];
+  uint64_t mma_done;  // the products of an MMA warp that gave up
   uint32_t tmem;
-  int abort;
   // (max, sum) of each row for the cluster's join: in q's memory, when the products are done
   __device__ __forceinline__ float2* ml(int t) { return reinterpret_cast<float2*>(q[0]) + t * BQ; }
 };
@@ -134,6 +134,12 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
   p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
   return p;
+}
+
+// mbar_wait of a warp that stays together: all lanes get the answer of all, so that a
+// wait that ran out for some of them takes every lane out of the same loop.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
 }
 
 // ---- thread-block clusters ----
@@ -207,7 +213,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
       mbar_init(&sm.l_full[t], 4);
       mbar_init(&sm.o_empty[t], 4);
     }
-    sm.abort = 0;
+    mbar_init(&sm.mma_done, 1);
     fence_barrier_init();
     fence_proxy_async();
   }
@@ -227,7 +233,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
     // ---------------- TMA producer ----------------
     give_registers<QT, EPILOGUE>();
     if (lane == 0) {
-      int slot = 0, items = 0;
+      int slot = 0, items = 0, q_loads[QT] = {};
       uint32_t phase = 0;
       bool ok = true;
       for (; ok && w.next(); ++items) {
@@ -235,9 +241,13 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
 #pragma unroll 1
           for (int v = 0; v < 2; ++v) {
             // q comes behind the first K, whose slot is free before the last item's q is
-            for (int t = 0; i == 0 && v == 1 && t < QT; ++t) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              if (i > 0 || v == 0) break;
               ok = ok && mbar_wait(&sm.q_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY);
-              if (ok) w.load_q(sm, &sm.q_full[t], t);
+              if (!ok) break;
+              w.load_q(sm, &sm.q_full[t], t);
+              ++q_loads[t];
             }
             if (!ok) break;
             if (!mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
@@ -253,14 +263,16 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           }
         }
       }
-      if (!ok) sm.abort = 1;
-      // Drain: every copy has landed and been consumed before the CTA leaves.
-      for (int s = 0; ok && s < SLOTS; ++s) {
-        mbar_wait(&sm.kv_empty[slot], phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
-        if (++slot == SLOTS) {
-          slot = 0;
-          phase ^= 1;
-        }
+      // Drain: every copy has landed and been consumed before the CTA leaves ..
+      for (int s = 0; ok && s < SLOTS; ++s)
+        ok = mbar_wait(&sm.kv_empty[s], s < slot ? phase : phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
+      // .. or, if a wait ran out, has landed at least: slots below `slot` were filled
+      // in this round of the ring, the others in the last one (parity 1 of a barrier
+      // that nothing was ever sent to is behind it).
+      if (!ok) {
+        for (int s = 0; s < SLOTS; ++s) mbar_wait(&sm.kv_full[s], s < slot ? phase : phase ^ 1, FB_KERR_TIMEOUT_FULL);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) mbar_wait(&sm.q_full[t], (q_loads[t] & 1) ^ 1, FB_KERR_TIMEOUT_FULL);
       }
     }
   } else if (warp == 4 * QT + 1) {
@@ -361,7 +373,10 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
       n = w.n;
       few = w.few;
     }
-    if (!ok) sm.abort = 1;
+    if (!ok) {  // no product is under way when the CTA frees its tensor memory
+      commit(&sm.mma_done);
+      warp_wait(&sm.mma_done, 0, FB_KERR_TIMEOUT_TMEM);
+    }
   } else if (warp < 4 * QT) {
     // ---------------- softmax + epilogue ----------------
     take_registers<QT, EPILOGUE>();
@@ -385,10 +400,11 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++tiles) {
         const int k0 = w.key0(i);
-        if (!mbar_wait(&sm.s_full[t], tiles & 1, FB_KERR_TIMEOUT_TMEM)) {
-          ok = false;
-          break;
-        }
+        // A wait that ran out is each lane's own until the next tile's vote, which is
+        // off the path from S to P: what the lane computes meanwhile is thrown away.
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ok = mbar_wait(&sm.s_full[t], tiles & 1, FB_KERR_TIMEOUT_TMEM);
         tc_fence_after();
         if (i == 0 && w.few) {
           // A few sinks far before the window: a tile of FEW keys.
@@ -440,7 +456,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           // is zeroed once the copy has landed (tile 0's P V runs first, so once is
           // enough).
           const uint32_t at = 2 * tiles + 1, slot = at % SLOTS;
-          if (!mbar_wait(&sm.kv_full[slot], (at / SLOTS) & 1, FB_KERR_TIMEOUT_FULL)) sm.abort = 1;
+          ok = mbar_wait(&sm.kv_full[slot], (at / SLOTS) & 1, FB_KERR_TIMEOUT_FULL) && ok;
           uint8_t* vrow = sm.kv[slot] + r * 128;
 #pragma unroll
           for (int e = 0; e < 16; ++e)  // (each lane from its own 16 bytes on: a warp's lanes in different banks)
@@ -503,7 +519,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
         if (EPILOGUE && i == n - 1) {
           // Not before the epilogue has read the last item's: with one key tile per
           // item nothing else would keep this warp from running two items ahead.
-          if (!mbar_wait(&sm.o_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_TMEM)) ok = false;
+          ok = mbar_wait(&sm.o_empty[t], (items & 1) ^ 1, FB_KERR_TIMEOUT_TMEM) && ok;
           sm.l[t][r] = l_run;
         }
         __syncwarp();
@@ -512,16 +528,16 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           if (EPILOGUE && i == n - 1) mbar_arrive(&sm.l_full[t]);
         }
       }
+      ok = __all_sync(0xffffffffu, ok);
       if constexpr (!EPILOGUE) {
         for (int i = 0; ok && n > 0 && i < QT; ++i)  // of every tile: a store may reuse the ring
-          if (i == t || Work::JOINS) ok = mbar_wait(&sm.o_full[i], items & 1, FB_KERR_TIMEOUT_TMEM);
+          if (i == t || Work::JOINS) ok = warp_wait(&sm.o_full[i], items & 1, FB_KERR_TIMEOUT_TMEM);
         if (ok) {
           tc_fence_after();
           w.store(sm, t, r, t_o, m_run, l_run, [] {});
         }
       }
     }
-    if (!ok) sm.abort = 1;
   } else if (EPILOGUE && warp >= 4 * QT + 4) {
     // ---------------- epilogue ----------------
     // O of an item is read while the softmax warps are at the next one.
@@ -536,7 +552,8 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
       for (int t = 0; ok && t < QT; ++t) {
         ok = mbar_wait(&sm.l_full[t], items & 1, FB_KERR_TIMEOUT_TMEM) &&
              mbar_wait(&sm.o_full[t], items & 1, FB_KERR_TIMEOUT_TMEM);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
         w.store(sm, t, r, tmem + (QT + t) * 128 + lane_base, 0.f, sm.l[t][r], [&] {
           tc_fence_before();
@@ -544,10 +561,10 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
           if (lane == 0) mbar_arrive(&sm.o_empty[t]);
         });
       }
-    if (!ok) sm.abort = 1;
   } else {
     give_registers<QT, EPILOGUE>();
   }
+  __syncwarp();  // the lane that copies is back with its warp
   w.finish(sm);
   tc_fence_before();
   __syncthreads();
