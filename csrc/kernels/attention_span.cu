@@ -66,6 +66,7 @@ struct Smem {
   uint8_t p[QP_BYTES];
   uint64_t kfull, vfull, kempty, vempty;
   uint64_t s_full, s_empty, p_full, o_full, o_empty;
+  uint64_t mma_done;  // the products of an MMA warp that gave up
   float red_max[4][NH], red_sum[4][NH];  // of a warp's tokens, for every head
   float mrun[2][NH];   // running max per head: one in use, one for the next move
   int scan[THREADS / 32];
@@ -238,6 +239,7 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
     mbar_init(&sm.s_empty, 4);
     mbar_init(&sm.p_full, 4);
     mbar_init(&sm.o_empty, 4);
+    mbar_init(&sm.mma_done, 1);
     sm.abort = sm.give_up = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -305,8 +307,9 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      uint32_t phase = 0;
-      for (Walk w(a, sm, begin, end); w.more() && !*(volatile int*)&sm.abort; w.next(a)) {
+      uint32_t loads[2] = {};  // of K and of V
+      bool ok = true;
+      for (Walk w(a, sm, begin, end); ok && w.more() && !*(volatile int*)&sm.abort; w.next(a)) {
         const int* bt = a.block_tables + static_cast<size_t>(w.b) * a.max_blocks;
         // Rows [16 * lo16, 16 * hi16) of a chunk's two pages and the pages' first cache row.
         auto chunk_pages = [&](int c, int (&lo16)[2], int (&hi16)[2], int (&rows)[2]) {
@@ -336,10 +339,9 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             uint64_t* full = kv ? &sm.vfull : &sm.kfull;
-            if (!mbar_wait(kv ? &sm.vempty : &sm.kempty, phase ^ 1, FB_KERR_TIMEOUT_EMPTY)) {
-              sm.abort = 1;
-              continue;  // no copies for this chunk; the loop ends below
-            }
+            ok = mbar_wait(kv ? &sm.vempty : &sm.kempty, (loads[kv] & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY);
+            if (!ok) break;
+            ++loads[kv];
             // An item's q rows come with its first K: the last item's Q K^T is done by then.
             const bool first = kv == 0 && c == w.c0;
             mbar_arrive_expect_tx(full, bytes + (first ? a.G * D * 2 : 0));
@@ -362,13 +364,18 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
               }
             }
           }
-          if (*(volatile int*)&sm.abort) break;
-          phase ^= 1;
+          if (!ok || *(volatile int*)&sm.abort) break;
         }
       }
-      // Drain: every issued copy has been consumed (or the kernel gave up).
-      mbar_wait(&sm.kempty, phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
-      mbar_wait(&sm.vempty, phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
+      // Drain: every issued copy has been consumed, or has landed at least where a
+      // wait ran out (parity 1 of a barrier that nothing was ever sent to is behind it).
+      ok = ok && mbar_wait(&sm.kempty, (loads[0] & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY) &&
+           mbar_wait(&sm.vempty, (loads[1] & 1) ^ 1, FB_KERR_TIMEOUT_EMPTY);
+      if (!ok) {
+        sm.abort = 1;
+        mbar_wait(&sm.kfull, (loads[0] & 1) ^ 1, FB_KERR_TIMEOUT_FULL);
+        mbar_wait(&sm.vfull, (loads[1] & 1) ^ 1, FB_KERR_TIMEOUT_FULL);
+      }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -409,7 +416,12 @@ __device__ __forceinline__ void span_body(const SpanMaps& maps, const Params& a)
           mma_commit(&sm.vempty);
         }
       }
-      if (!ok) sm.abort = 1;
+      if (!ok) {
+        sm.abort = 1;
+        // no product is under way when the CTA frees its tensor memory
+        mma_commit(&sm.mma_done);
+        mbar_wait(&sm.mma_done, 0, FB_KERR_TIMEOUT_TMEM);
+      }
     }
   } else {
     // ---------------- softmax / epilogue (warps 2..5) ----------------

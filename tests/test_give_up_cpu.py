@@ -76,3 +76,20 @@ def test_ring_drain_waits_for_every_copy_that_was_issued():
     for loads in range(5):
         parity = (loads & 1) ^ 1
         assert (loads & 1) != parity and (not loads or (loads - 1 & 1) == parity)
+
+
+def test_span_kernel_waits_for_what_is_under_way():
+    text = _source("attention_span.cu")
+    copies = _body(text, "if (warp == 0)")
+    empty = copies.index("ok = mbar_wait(kv ? &sm.vempty : &sm.kempty")
+    # behind a wait that ran out no further copy is issued ..
+    assert copies.index("if (!ok) break;") < copies.index("++loads[kv];") < copies.index("tma_load")
+    assert empty < copies.index("if (!ok) break;") and "continue;\n            }" not in copies
+    # .. and those that were have landed before the block leaves
+    drain = _body(copies[copies.rindex("if (!ok) {"):], "if (!ok)")
+    for which, at in (("k", 0), ("v", 1)):
+        assert f"mbar_wait(&sm.{which}full, (loads[{at}] & 1) ^ 1" in drain
+        assert f"mbar_wait(&sm.{which}empty, (loads[{at}] & 1) ^ 1" in copies
+    mma = _body(text, "else if (warp == 1)")
+    drain = _body(mma[mma.rindex("if (!ok) {"):], "if (!ok)")
+    assert drain.index("mma_commit(&sm.mma_done)") < drain.index("mbar_wait(&sm.mma_done, 0")
