@@ -192,16 +192,87 @@ _CLUSTERS = {1: 148, 2: 72, 3: 44, 4: 32, 5: 24, 6: 16, 7: 14, 8: 13}
 _PREFIX_LEAST_US = 7.0  # of the prefix kernel: start, end and join
 
 
-def _prefix_us(clusters: int, pages: int, tiles: int, cluster: int, parts: int, sms: int) -> float:
-    """Estimated microseconds of the prefix kernel: ``clusters`` (query tiles x KV
-    heads) times ``parts`` clusters of ``cluster`` CTAs, which have an equal part
-    of the pages each. Measured on 148 SMs: 2.1 us per key tile with two query
-    tiles per CTA, 2.2 with two CTAs per SM, 1.8 with one, and 7 us for start,
-    end and join; 0.7 us per further part in the kernel that goes on from them."""
-    held = max(1, _CLUSTERS[cluster] * (3 - tiles) * sms // 148)
-    step = 2.1 if tiles == 2 else 2.2 if clusters * parts * cluster > sms else 1.8
-    keys = -(-((pages + 1) // 2) // (cluster * parts))
-    return -(-clusters * parts // held) * (keys * step + _PREFIX_LEAST_US) + 0.7 * (parts - 1)
+def _prefix_us(kinds: list[tuple[int, int]], tiles: int, cluster: int, parts: int, sms: int) -> float:
+    """Estimated microseconds of the prefix kernel for ``kinds`` of (key tiles,
+    query tiles x KV heads), the longest first: ``parts`` clusters of ``cluster``
+    CTAs for each query tile, which have an equal part of the keys each. Measured
+    on 148 SMs: 2.1 us per key tile with two query tiles per CTA, 2.2 with two
+    CTAs per SM, 1.8 with one, and 7 us for start, end and join; 0.7 us per further
+    part in the kernel that goes on from them. Clusters run in waves of as many as
+    the SMs hold, a wave as long as its longest cluster.
+
+    Clusters of different lengths are not started longest first, KV head by KV
+    head: 12 us per further wave and 8 per further part came closest to the best
+    of all shapes in 11 measured mixtures (4% above it, at most 22%; 10% and 43%
+    with every cluster taken for as long as the longest)."""
+    held, splits = _clusters_held(tiles, cluster, sms), cluster * parts
+    step = _step_us(tiles, sum(n for _, n in kinds) * splits, sms)
+    wave, part = (12.0, 8.0) if kinds[0][0] != kinds[-1][0] else (0.0, 0.7)
+    us, clusters, waves = part * (parts - 1) - wave, 0, 0
+    for keys, n in kinds:
+        clusters += n * parts
+        begun = -(-clusters // held)
+        if begun > waves:
+            us += (begun - waves) * (-(-keys // splits) * step + _PREFIX_LEAST_US + wave)
+            waves = begun
+    return us
+
+
+def _clusters_held(tiles: int, cluster: int, sms: int) -> int:
+    return max(1, _CLUSTERS[cluster] * (3 - tiles) * sms // 148)
+
+
+def _step_us(tiles: int, ctas: int, sms: int) -> float:
+    return 2.1 if tiles == 2 else 2.2 if ctas > sms else 1.8
+
+
+def _few_bits(x: int) -> int:
+    """x rounded up to three significant bits."""
+    low = max(0, x.bit_length() - 3)
+    return -(-x >> low) << low
+
+
+def _share(groups: list[tuple[int, int]], group: int, n_kv: int, share: bool | None) -> tuple[set, int, int, int]:
+    """(the (rows, pages) to share, query tiles per CTA, cluster size, parts) with
+    the least estimated time of the prefix kernel and of reading the other groups'
+    prefixes row by row. ``share`` True: all of them, None: those that are worth it."""
+    nb, sms, longest = prefix_rows(group), _rt.sm_count(), max((p + 1) // 2 for _, p in groups)
+    # kinds of groups: (rows, key tiles) -> [groups, us to read them row by row at 85% of the HBM rate, (rows, pages)]
+    kinds: dict = {}
+    coarse = len(set(groups)) > 64  # many different ones: alike to a few bits are alike, so that the search stays short
+    for n, p in groups:
+        keys = (p + 1) // 2
+        kind = kinds.setdefault((_few_bits(n), _few_bits(keys)) if coarse else (n, keys), [0, 0.0, set()])
+        kind[0] += 1
+        kind[1] += n * p * PAGE * n_kv * 512 / 5.5e6
+        kind[2].add((n, p))
+    kinds = sorted(((keys, n, count, us, which) for (n, keys), (count, us, which) in kinds.items()),
+                   key=lambda kind: -kind[0])
+    again = sum(kind[3] for kind in kinds)
+    if not share and again <= _PREFIX_LEAST_US:
+        return set(), 1, 1, 1
+    best, mixed = (math.inf if share else again, 1, 1, 1, []), not share and len(kinds) > 1
+    for t in (1, 2):
+        work = [(keys, n_kv * count * -(-n // (nb * t))) for keys, n, count, _, _ in kinds]
+        step = _step_us(t, sms + 1, sms)
+        for c in _CLUSTERS:
+            held = _clusters_held(t, c, sms)
+            for p in (1, 2, 4, 8):
+                if c * p > max(1, longest):
+                    break
+                us = _prefix_us(work, t, c, p, sms)
+                if us < best[0]:
+                    best = us, t, c, p, kinds
+                if not mixed:
+                    continue
+                # without the kinds that save less than their part of the SMs' time
+                paid = [i for i, (keys, n) in enumerate(work) if kinds[i][3] > n * p * (
+                    -(-keys // (c * p)) * step + _PREFIX_LEAST_US) / held]
+                if 0 < len(paid) < len(kinds):
+                    us = _prefix_us([work[i] for i in paid], t, c, p, sms) + again - sum(kinds[i][3] for i in paid)
+                    if us < best[0]:
+                        best = us, t, c, p, [kinds[i] for i in paid]
+    return {g for kind in best[4] for g in kind[4]}, *best[1:4]
 
 
 class PrefixPlan:
@@ -215,8 +286,8 @@ class PrefixPlan:
     it has to outlive them.
 
     Groups that are too small, or prefixes too short, for the shared pages'
-    extra kernel to pay are read row by row (``share=None``: by an estimate of
-    both; True and False decide for it)."""
+    extra kernel to pay are read row by row (``share=None``: each group by an
+    estimate of both; True and False decide for all)."""
 
     def __init__(self, group_sizes: list[int], prefix_pages: list[int], n_q: int, n_kv: int, max_blocks: int,
                  arena=None, device=None, share: bool | None = None):
@@ -231,21 +302,14 @@ class PrefixPlan:
         self.n_q, self.n_kv, self.max_blocks = n_q, n_kv, max_blocks
         self.rows = sum(group_sizes)
         least = 1 if share else 2  # rows that can share anything
-        shared = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n >= least and p]
-        nb, sms, longest = prefix_rows(group), _rt.sm_count(), max((p for _, p in shared), default=0)
-        us, self.tiles, self.cluster, self.parts = 0.0, 1, 1, 1
-        again = sum(n * p for n, p in shared) * PAGE * n_kv * 512 / 5.5e6  # us row by row, at 85% of the HBM rate
-        if shared and (share or share is None and again > _PREFIX_LEAST_US):
-            us, self.tiles, self.cluster, self.parts = min(
-                (_prefix_us(clusters, longest, t, c, p, sms), t, c, p)
-                for t, clusters in ((t, n_kv * sum(-(-n // (nb * t)) for n, _ in shared)) for t in (1, 2))
-                for c in _CLUSTERS for p in (1, 2, 4, 8) if c * p <= max(1, (longest + 1) // 2))
-        if share is None:
-            share = again > max(us, _PREFIX_LEAST_US)
-        splits = self.cluster * self.parts
+        groups = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n >= least and p]
+        shared, self.tiles, self.cluster, self.parts = set(), 1, 1, 1
+        if groups and share is not False:
+            shared, self.tiles, self.cluster, self.parts = _share(groups, group, n_kv, share)
+        nb, splits = prefix_rows(group), self.cluster * self.parts
         items, info, row = [], [], 0
         for n, pages in zip(group_sizes, prefix_pages):
-            is_shared = share and n >= least and pages > 0
+            is_shared = n >= least and (n, pages) in shared
             if is_shared:
                 keys = math.ceil(pages / 2)
                 cuts = [min(2 * (keys * s // splits), pages) for s in range(splits + 1)]
