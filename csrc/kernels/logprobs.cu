@@ -13,11 +13,12 @@
 // below. Only the parts of threads whose max reaches that bound - about k of
 // them, but for ties - are read again (from L2, by the whole block), and what
 // reaches the bound is listed; the list, rarely longer than 2 k, is ranked by
-// counting. Two ways out keep that exact for any input: more equal logits at
-// the bound than the list holds are taken in token order, 256 at a time until
-// enough are found (a constant row ends in its first step); more logits above
-// the bound than the list holds (few threads' parts hold many of the largest)
-// are found by k passes.
+// counting. Two ways out keep that exact for any input: with more than 256 on the
+// list, those above the bound are listed alone, and of the equal ones at it the
+// first in token order are taken, 256 logits at a time until enough are found (a
+// constant row, or one masked but for a few tokens, ends in its first step); more
+// logits above the bound than the list holds (few threads' parts hold many of the
+// largest) are found by k passes.
 //
 // The kernel is bound by reading the logits (bf16: by one 2^x per 2 bytes
 // almost as much: 16 a clock and SM against 11.5 that HBM delivers). Each thread
@@ -33,7 +34,8 @@
 //
 // Measured (B200): 2000 x 151936 fp32, k = 1 197 us (94% of the 6545 GB/s of a plain
 // copy), bf16 125 us (74%); 256 x 128256 bf16, k = 0 / 5 / 20 16.7 / 19.2 / 21.3 us
-// (3.9 / 3.4 / 3.1 TB/s: two rows on most SMs, 1.73 on average); one row, k = 5 8.7 us.
+// (3.9 / 3.4 / 3.1 TB/s: two rows on most SMs, 1.73 on average), of which constant
+// rows 27 us and rows masked but for three tokens 42 us; one row, k = 5 8.7 us.
 #include <cuda_fp16.h>
 
 #include "fb_common.cuh"
@@ -48,6 +50,7 @@ constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_K = 32;
 constexpr int LIST = 1024;   // logits that reach the bound
+constexpr int PLAIN = 256;   // so many are ranked as they are; of more, first those above the bound
 constexpr int MAX_PIECES = 1024;  // of a row: at most the grid, and two
 constexpr int GROUPS = 64;            // of THREADS / GROUPS neighbouring threads
 constexpr int U = 4;          // vectors that a thread works on at a time
@@ -295,6 +298,7 @@ __device__ __noinline__ void piece_top(const T* x, int n, int head, int vecs, in
   __syncthreads();
   // Lists what reaches the bound (or, with `above`, passes it): the listed
   // threads' vectors come back into the ring, as many as it holds at a time.
+  // Ends as soon as there is more than the list holds.
   auto collect = [&](bool above) {
     auto look = [&](float f, int i) {
       if (f > bound || (f == bound && !above)) {
@@ -325,23 +329,24 @@ __device__ __noinline__ void piece_top(const T* x, int n, int head, int vecs, in
         if (tid == 0) sm.n_hit = 0;
         copy_wait<0>();
         __syncthreads();
-        each([&](int at, int slot) {  // vectors that reach the bound ..
+        each([&](int at, int slot) {  // vectors that reach (pass) the bound ..
           float f[N];
           Vec<T>::unpack(ring[slot], f);
           float mx = f[0];
 #pragma unroll
           for (int e = 1; e < N; ++e) mx = fmaxf(mx, f[e]);
-          if (mx >= bound)
+          if (above ? mx > bound : mx >= bound)
             if (const int i = atomicAdd(&sm.n_hit, 1); i < LIST) sm.hit[i] = make_int2(at, slot);
         });
         __syncthreads();
         const int hits = sm.n_hit;
-        if (hits > LIST && tid == 0) sm.n_list = LIST + 1;  // more logits than that, too
+        if (hits > LIST && tid == 0) atomicAdd(&sm.n_list, LIST + 1);  // more logits than that, too
         for (int i = tid; i < min(hits, LIST) * N; i += THREADS) {  // .. and their logits, one to a thread
           const int2 h = sm.hit[i / N];
           look(to_float(reinterpret_cast<const T*>(ring + h.y)[i % N]), head + h.x * N + i % N);
         }
         __syncthreads();
+        if (sm.n_list > LIST) return;  // (the same in all threads: written again behind the next barrier)
       }
     }
     __syncthreads();
@@ -350,15 +355,41 @@ __device__ __noinline__ void piece_top(const T* x, int n, int head, int vecs, in
     if (rank < k) sm.best[rank] = sm.list[i];
   };
   collect(false);
-  if (sm.n_list <= LIST) {
-    rank_keys(sm.list, sm.n_list, keep);
+  const int listed = sm.n_list;
+  bool ties = listed > LIST;
+  if (listed > PLAIN && !ties) {  // ties at the bound, or many different logits above it?
+    unsigned long long mine[LIST / THREADS];
+    int more = 0;
+    const unsigned long long at_bound = static_cast<unsigned long long>(ordered(bound)) << 32 | 0xffffffffu;
+#pragma unroll
+    for (int q = 0; q < LIST / THREADS; ++q) {
+      mine[q] = tid + q * THREADS < listed ? sm.list[tid + q * THREADS] : 0;
+      more += __syncthreads_count(mine[q] > at_bound);
+    }
+    ties = more <= PLAIN;
+    if (ties) {
+      if (tid == 0) sm.n_list = 0;
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < LIST / THREADS; ++q)
+        if (mine[q] > at_bound) sm.list[atomicAdd(&sm.n_list, 1)] = mine[q];
+      __syncthreads();
+    }
+  } else if (ties) {
+    // Ties, or masked logits where fewer than k groups have others: only what is
+    // above the bound is worth listing.
+    __syncthreads();
+    if (tid == 0) sm.n_list = sm.n_listed = 0;
+    __syncthreads();
+    if (tmax > bound) sm.listed[atomicAdd(&sm.n_listed, 1)] = static_cast<unsigned char>(tid);
+    __syncthreads();
+    collect(true);
+  }
+  if (!ties) {
+    rank_keys(sm.list, listed, keep);
     __syncthreads();
     return;
   }
-  __syncthreads();
-  if (tid == 0) sm.n_list = 0;
-  __syncthreads();
-  collect(true);
   if (sm.n_list <= LIST) {
     int found = sm.n_list;
     rank_keys(sm.list, found, keep);
