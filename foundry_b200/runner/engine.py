@@ -20,6 +20,7 @@ python/foundry/integration/vllm/graph_ops.py:123-205 capture-or-load loop).
 from __future__ import annotations
 
 import math
+import operator
 import threading
 import time
 from dataclasses import dataclass, field
@@ -486,8 +487,9 @@ class LLMEngine:
         vocabulary sharded over tensor-parallel ranks."""
         if self.tp is not None:
             raise ValueError("log probabilities need the whole vocabulary on this rank (tp = 1)")
-        if not 0 <= top <= min(MAX_TOP, self.weights.vocab_l):
-            raise ValueError(f"top must be 0 to {min(MAX_TOP, self.weights.vocab_l)}, got {top}")
+        most = min(MAX_TOP, self.weights.vocab_l)
+        if not hasattr(top, "__index__") or not 0 <= (top := operator.index(top)) <= most:
+            raise ValueError(f"top must be a whole number from 0 to {most}, got {top!r}")
         reqs = self._generate(prompts, max_new_tokens, top)
         return [r.output for r in reqs], [r.logprobs for r in reqs]
 
