@@ -565,11 +565,13 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
     give_registers<QT, EPILOGUE>();
   }
   __syncwarp();  // the lane that copies is back with its warp
-  w.finish(sm);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Before a cluster's join: a CTA that waits for another one, which may itself be
+  // waiting for tensor memory, holds none.
   if (warp == 4 * QT + 1) tmem_dealloc(tmem, QT * 256);
+  w.finish(sm);
 }
 
 template <class Smem>

@@ -93,3 +93,11 @@ def test_span_kernel_waits_for_what_is_under_way():
     mma = _body(text, "else if (warp == 1)")
     drain = _body(mma[mma.rindex("if (!ok) {"):], "if (!ok)")
     assert drain.index("mma_commit(&sm.mma_done)") < drain.index("mbar_wait(&sm.mma_done, 0")
+
+
+def test_clusters_hold_no_tensor_memory_while_they_wait_for_each_other():
+    """A CTA of a cluster that keeps its tensor memory until the others have come,
+    one of which waits for tensor memory that another kernel's cluster holds in the
+    same way, would wait for good."""
+    body = _body(_source("attention_tile.cu"), "void tile_attention(")
+    assert body.index("tmem_dealloc(") < body.index("w.finish(sm)") and "cluster_sync" not in body
