@@ -48,8 +48,8 @@ def _check_device(*tensors: torch.Tensor) -> int:
 def _check_scale(scale: float | None) -> float:
     if scale is None:
         return 1.0 / math.sqrt(128)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"scale must be positive, got {scale}")
+    if not 2.0**-120 <= scale <= 2.0**120:  # (NaN is neither; beyond, fp32 holds it as zero or not at all)
+        raise ValueError(f"scale must be positive and in fp32's range, got {scale}")
     return float(scale)
 
 

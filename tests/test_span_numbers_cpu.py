@@ -57,3 +57,28 @@ def test_plan_takes_whole_rows_and_pages():
     for sizes, pages in ((np.array([3, 2]), np.array([2, 4])), (torch.tensor([3, 2]), torch.tensor([2, 4]))):
         plan = ops.PrefixPlan(sizes, pages, 8, 2, 4, device="cpu", share=True)
         assert plan.rows == 5 and torch.equal(plan.items, want.items) and torch.equal(plan.row_prefix, want.row_prefix)
+
+
+@pytest.mark.parametrize("scale", [1e-45, 1e-38, 1e38, 1e300, float("inf"), float("nan"), 0.0, -0.1])
+def test_scale_that_fp32_does_not_hold(launches, scale):
+    """Times log2(e) it would be zero (masked scores: -inf * 0), infinite or subnormal in the kernel."""
+    q, cache = torch.zeros(3, 8, 128, dtype=torch.bfloat16), torch.zeros(10, 2, 64, 128, dtype=torch.bfloat16)
+    kv, tiles = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    args = q, cache, cache, torch.zeros(3, 4, dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.zeros_like(q)
+    plan = ops.PrefixPlan([3], [2], 8, 2, 4, device="cpu", share=True)
+    ws = ops.SpanWorkspace(plan.partials, device="cpu")
+
+    def calls(scale):
+        yield lambda: ops.window_decode_attention(*args, 64, 0, ws, scale=scale)
+        yield lambda: ops.prefix_decode_attention(*args, plan, ws, scale=scale)
+        yield lambda: ops.window_prefill_attention(q.view(3, 1024), kv, kv, torch.zeros(3, 1024, dtype=torch.bfloat16),
+                                                   torch.tensor([0, 3], dtype=torch.int32), tiles, tiles, 8, 2, 64, 0,
+                                                   scale=scale)
+
+    for call in calls(scale):
+        with pytest.raises(ValueError, match="scale"):
+            call()
+    assert not launches
+    for fine in (None, 1, 0.0883, 1e-30, 1e30):
+        for call in calls(fine):
+            call()
