@@ -23,8 +23,11 @@
 //                      for it), V MN-major from the image that TMA wrote
 // A CTA holds QT query tiles: with QT = 2 they share every K/V tile and take
 // turns, the tensor cores working on one tile's products while the other's
-// 128 threads do its softmax; QT = 1 (half the shared memory and TMEM, two
-// CTAs per SM) is for work with no second tile. TMEM: QT x (128 columns S/P +
+// 128 threads do its softmax; QT = 1 has half the shared memory and TMEM, and two
+// CTAs per SM. A prefill's two tiles are two heads of one KV head: with an odd
+// number of them, QT = 1. (Heads 32 / 8: 154 us with QT = 2, 216 with QT = 1 on 8192
+// tokens, 47 and 64 on short prompts; 24 / 8, which has only QT = 1, 162 and 49.)
+// The prefix kernel takes either, by the estimate of PrefixPlan. TMEM: QT x (128 columns S/P +
 // 128 columns O).
 //
 // The MMA thread issues P_t V_i and then Q_t K_{i+1}, which overwrites P_t's
@@ -34,18 +37,21 @@
 // 8 (log2 units; p stays below 256, exact in the fp32 sum), so O is rarely
 // rescaled.
 //
-// p is rounded to bf16 for the second product (half a step: relative 2^-9 of
-// each term, with random signs), the sum l and both products accumulate in fp32.
+// p is rounded to bf16 for the second product (half a step: relative 2^-8 of
+// each term, with random signs), as much as the output's own rounding; the sum l
+// is of the unrounded p, and it and both products accumulate in fp32.
 //
 // Roles: 4 QT softmax warps (a thread per query row), one TMA warp, one MMA warp,
 // and for the two-tile prefill four warps that normalise and store an item's O
 // while the softmax warps are at the next item (two more fill their warpgroup);
 // elsewhere the softmax warps do that. With QT = 2 the other warps give registers
-// to the softmax warps, which hold 128 scores each.
+// to the softmax warps, which hold 128 scores each; even so each variant spills a
+// few registers (24 to 200 bytes of stores a thread).
 //
 // Measured (B200): prefill of 8192 tokens, 32 / 8 heads, window 1024 and 4 sinks
-// 160 us (129 GFLOP of visible pairs: 807 TFLOP/s); 13 prompts of 1 to 700 tokens,
-// window 128 48 us. Prefix of 32768 tokens for 128 rows of 64 / 8 heads 133 us
+// 154 to 163 us (129 GFLOP of visible pairs: 840 to 795 TFLOP/s), 184 us (700) where
+// repeated calls bring the clocks down to the power cap; 13 prompts of 1 to 700
+// tokens, window 128 48 us. Prefix of 32768 tokens for 128 rows of 64 / 8 heads 133 us
 // (137 GFLOP, 1030 TFLOP/s); of 2048 tokens for 256 rows of 32 / 8 heads 21 us.
 // Bound by the chain of a step rather than by a pipe: softmax 1900 clocks, signal
 // to the MMA warp 440, P V and the next Q K^T 1020; two query tiles overlap their
@@ -115,7 +121,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // unit gives 16 exponentials a clock and SM, as many as the two products of a tile
 // take time for; some on the FMA pipes bring the softmax below the products.
 // x = n + f, |f| <= 1/2; 2^f by the polynomial of degree 4 with the least relative
-// error (2.7e-6, found by linear programming; p is rounded to 2^-9 next). x below
+// error (2.7e-6, found by linear programming; p is rounded to 2^-8 next, and
+// the sum l, which takes it as it is, is off by no more than that). x below
 // -126 gives 2^-126 at least, and so does NaN: the caller sees to it that the sum
 // of a row with such a score is NaN.
 constexpr int POLY_OF = 4;

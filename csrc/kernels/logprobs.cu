@@ -20,8 +20,11 @@
 // logits above the bound than the list holds (few threads' parts hold many of the
 // largest) are found by k passes.
 //
-// The kernel is bound by reading the logits (bf16: by one 2^x per 2 bytes
-// almost as much: 16 a clock and SM against 11.5 that HBM delivers). Each thread
+// With k = 0 the kernel is bound by reading the logits (2000 x 151936: fp32 all of a
+// plain copy's rate, bf16 85%: one 2^x per 2 bytes takes 72% of what the
+// special-function units give at that rate). The choice of the k largest comes at a
+// row's end, while its CTA reads nothing: 2000 rows in bf16, k = 0 / 1 / 20 109 / 127 /
+// 159 us. Each thread
 // copies its next 128 bytes into its own slots of shared memory while it works on
 // 64, which takes neither registers nor barriers. (Slower: loads ahead into
 // registers, which spill; a ring of bulk copies for the block, whose barriers cost
@@ -32,8 +35,8 @@
 // per CTA and one ticket per cut (zero before and after every launch). The join is
 // in piece order, so results do not depend on which CTA comes last.
 //
-// Measured (B200): 2000 x 151936 fp32, k = 1 197 us (94% of the 6545 GB/s of a plain
-// copy), bf16 125 us (74%); 256 x 128256 bf16, k = 0 / 5 / 20 16.7 / 19.2 / 21.3 us
+// Measured (B200): 2000 x 151936, k = 1: fp32 185 us in a graph, 197 call by call (94%
+// of the 6545 GB/s of a plain copy), bf16 127 us (73%), fp16 125 us; 256 x 128256 bf16, k = 0 / 5 / 20 16.7 / 19.2 / 21.3 us
 // (3.9 / 3.4 / 3.1 TB/s: two rows on most SMs, 1.73 on average), of which constant
 // rows 27 us and rows masked but for three tokens 42 us; one row, k = 5 8.7 us.
 #include <cuda_fp16.h>
