@@ -203,8 +203,8 @@ def _prefix_us(kinds: list[tuple[int, int]], tiles: int, cluster: int, parts: in
 
     Clusters of different lengths are not started longest first, KV head by KV
     head: 12 us per further wave and 8 per further part came closest to the best
-    of all shapes in 11 measured mixtures (4% above it, at most 22%; 10% and 43%
-    with every cluster taken for as long as the longest)."""
+    of all shapes in 12 measured mixtures (6% above it on average, at most 22%; 15%
+    and 43% with every cluster taken for as long as the longest)."""
     held, splits = _clusters_held(tiles, cluster, sms), cluster * parts
     step = _step_us(tiles, sum(n for _, n in kinds) * splits, sms)
     wave, part = (12.0, 8.0) if kinds[0][0] != kinds[-1][0] else (0.0, 0.7)
