@@ -304,7 +304,7 @@ class PrefixPlan:
         least = 1 if share else 2  # rows that can share anything
         groups = [(n, p) for n, p in zip(group_sizes, prefix_pages) if n >= least and p]
         shared, self.tiles, self.cluster, self.parts = set(), 1, 1, 1
-        if groups and share is not False:
+        if groups and (share is None or share):
             shared, self.tiles, self.cluster, self.parts = _share(groups, group, n_kv, share)
         nb, splits = prefix_rows(group), self.cluster * self.parts
         items, info, row = [], [], 0

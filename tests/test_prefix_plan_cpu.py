@@ -101,3 +101,11 @@ def test_many_different_groups_are_planned_at_once():
     t = time.perf_counter()
     plan = _plan(groups)
     assert plan.items_n and time.perf_counter() - t < 2.0  # 0.1 s here
+
+
+def test_share_is_a_truth_value_or_none():
+    groups = [(100, 300)]
+    for no in (False, 0, torch.tensor(False)):
+        assert not _plan(groups, share=no).items_n
+    for yes in (True, 1, torch.tensor(True)):
+        assert _plan([(2, 1)], share=yes).items_n
