@@ -274,7 +274,7 @@ __device__ __forceinline__ void tile_attention(Work w, Smem& sm, float scale_log
       for (int s = 0; ok && s < SLOTS; ++s)
         ok = mbar_wait(&sm.kv_empty[s], s < slot ? phase : phase ^ 1, FB_KERR_TIMEOUT_EMPTY);
       // .. or, if a wait ran out, has landed at least: slots below `slot` were filled
-      // in this round of the ring, the others in the last one (parity 1 of a barrier
+      // in this turn of the ring, the others in the last one (parity 1 of a barrier
       // that nothing was ever sent to is behind it).
       if (!ok) {
         for (int s = 0; s < SLOTS; ++s) mbar_wait(&sm.kv_full[s], s < slot ? phase : phase ^ 1, FB_KERR_TIMEOUT_FULL);
